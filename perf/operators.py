@@ -110,10 +110,11 @@ def _encode(x):
     """Codes (uint8, one per value) and (scale, lo) in f32 of rows of f32 values."""
     lo, span = x.amin(-1), x.amax(-1) - x.amin(-1)
     flat = span < TINY
-    rate = 15.0 / torch.where(flat, torch.ones_like(span), span)
+    fifteen = torch.full_like(span, 15.0)  # tensor by tensor: divisions by or of a number do not round once
+    rate = fifteen / torch.where(flat, torch.ones_like(span), span)
     code = torch.round((x - lo[..., None]) * rate[..., None]).clamp(max=15.0)
     code = torch.where(flat[..., None], torch.zeros_like(code), code)
-    return code.to(torch.uint8), torch.where(flat, torch.zeros_like(span), span / 15.0), lo
+    return code.to(torch.uint8), torch.where(flat, torch.zeros_like(span), span / fifteen), lo
 
 
 def _records(k, v):
@@ -304,8 +305,10 @@ def _stored64(x):
     hi, lo = x32.max(-1, keepdim=True).values, x32.min(-1, keepdim=True).values
     span = hi - lo
     dead = span < 2.0 ** -100
-    code = ((x32 - lo) * (15.0 / span.masked_fill(dead, 1.0))).round().double().clamp(0, 15)
-    return torch.where(dead, lo.double(), lo.double() + (span / 15.0).double() * code)
+    # f64 quotients of f32 values, rounded once more to f32, are the f32 quotients.
+    rate = (15.0 / span.masked_fill(dead, 1.0).double()).float()
+    code = ((x32 - lo) * rate).round().double().clamp(0, 15)
+    return torch.where(dead, lo.double(), lo.double() + (span.double() / 15.0).float().double() * code)
 
 
 def _record64(rec, at, d):
