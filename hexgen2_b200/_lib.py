@@ -59,6 +59,24 @@ _SIGNATURES = {
                                             c_int64, c_int64, c_int64, c_int64, c_float, c_void_p,
                                             c_int, c_void_p]),
     "hx_argmax": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "hx_quantize_cache_q4": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                     c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                     c_int64, c_int64, c_int, c_void_p]),
+    "hx_dequantize_cache_q4": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                       c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                                       c_int64, c_int64, c_int, c_void_p]),
+    "hx_rotary_cache_write_q4": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                         c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p,
+                                         c_void_p, c_int64, c_int64, c_int64, c_int64, c_int,
+                                         c_void_p]),
+    "hx_decode_attention_q4": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p,
+                                       c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
+                                       c_void_p, c_void_p, c_size_t, c_int, c_void_p]),
+    "hx_decode_attention_q4_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "hx_gemm_q4": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
+                           c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int, c_void_p]),
+    "hx_token_logprobs": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "hx_kv_pack": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                            c_int64, c_int64, c_void_p, c_void_p]),
     "hx_kv_unpack": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,

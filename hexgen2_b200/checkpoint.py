@@ -151,6 +151,29 @@ def shard_state_dict_tp(state_dict: dict, config, world_size: int, rank: int) ->
     return sd
 
 
+def quantize_weight_q4(w: torch.Tensor, group: int = 128):
+    """A weight [N, K] in 4 bits with group scales, as ops.gemm_q4 takes it: (codes uint8 [N, K / 2],
+    element 2j in the low nibble of byte j; scales [N, K / group] in w's dtype), for
+    w ~ scale * (code - 8) with scale = max |w| / 7 of the group. Rows keep their order, so an
+    interleaved fc1 (gpt.interleave_gated) stays one."""
+    if w.dim() != 2 or group not in (32, 64, 128) or w.shape[1] % group:
+        raise ValueError(f"quantize_weight_q4: weight {tuple(w.shape)} in groups of {group} (32, 64 or 128)")
+    n, k = w.shape
+    x = w.detach().float().view(n, k // group, group)
+    scales = (x.abs().amax(-1) / 7.0).to(w.dtype)
+    step = scales.float()[..., None]
+    codes = torch.where(step > 0, torch.round(x / step), torch.zeros_like(x)).clamp(-8, 7) + 8
+    codes = codes.to(torch.uint8).view(n, k)
+    return codes[:, 0::2] | codes[:, 1::2] << 4, scales
+
+
+def dequantize_weight_q4(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The weight [N, K] that quantize_weight_q4's codes and scales stand for, in f32."""
+    n, k = codes.shape[0], 2 * codes.shape[1]
+    x = torch.stack((codes & 15, codes >> 4), -1).view(n, scales.shape[1], -1).float() - 8.0
+    return (x * scales.float()[..., None]).view(n, k)
+
+
 def load_safetensors_dir(model_dir) -> dict:
     """All *.safetensors shards of a checkpoint; duplicate keys are an error (model.py:58-66)."""
     from safetensors.torch import load_file

@@ -6,6 +6,8 @@ per-device buffer that grows on demand and is reused across calls on the same st
 """
 from __future__ import annotations
 
+from collections import namedtuple
+
 import torch
 
 from . import _lib
@@ -69,6 +71,31 @@ def workspace(nbytes: int, device=None, kind: str = "attn") -> torch.Tensor | No
         _workspaces[key] = buf
         WORKSPACE_GEN += 1
     return buf
+
+
+def _device_of(*ts) -> int:
+    """The one CUDA device that all of the given tensors are on."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("hexgen2_b200 kernels take CUDA tensors (there is no CPU path)")
+        if dev is None:
+            dev = t.get_device()
+        elif t.get_device() != dev:
+            raise ValueError("all tensors of a call must be on the same device")
+    return dev
+
+
+def _call(dev: int, name: str, *args):
+    """Calls entry point `name` with the current stream of device `dev`, whichever device is
+    current."""
+    if dev == torch.cuda.current_device():
+        check(getattr(_L(), name)(*args, _stream()), name)
+    else:
+        with torch.cuda.device(dev):
+            check(getattr(_L(), name)(*args, _stream()), name)
 
 
 # ----------------------------------------------------------------------------- norms
@@ -283,6 +310,185 @@ def decode_workspace_bytes(batch, n_heads, head_dim, max_seqlen) -> int:
     return _L().hx_decode_attention_workspace(batch, n_heads, head_dim, max_seqlen)
 
 
+# ----------------------------------------------------------------------------- 4-bit KV cache
+Q4_META_BYTES = 16  # k_scale, k_min, v_scale, v_min (f32) behind the codes of a record
+
+
+def allocate_cache_q4(batch, n_heads_kv, max_seqlen, head_dim, device=None) -> torch.Tensor:
+    """A KV cache of one layer held in 4 bits: uint8 [batch, n_heads_kv, max_seqlen, head_dim + 16],
+    one record (K codes, V codes, scales and minima) per position and KV head, 144 bytes where 16
+    bits take 512 (head_dim 128). The format is described at hx_quantize_cache_q4."""
+    return torch.empty(batch, n_heads_kv, max_seqlen, head_dim + Q4_META_BYTES, dtype=torch.uint8,
+                       device="cuda" if device is None else device)
+
+
+def _check_q4(what, cache_q4, n_heads_kv, head_dim, first=0, batch=0, written=False):
+    if cache_q4.dtype != torch.uint8 or cache_q4.dim() != 4:
+        raise ValueError(f"{what}: the 4-bit cache is uint8 [batch, kv heads, positions, head_dim + 16]")
+    shape, stride = cache_q4.shape, cache_q4.stride()
+    if shape[1] != n_heads_kv or shape[3] != head_dim + Q4_META_BYTES:
+        raise ValueError(f"{what}: 4-bit cache of shape {tuple(shape)} for {n_heads_kv} KV heads of {head_dim}")
+    if stride[3] != 1 or stride[2] != shape[3]:
+        raise ValueError(f"{what}: the records of a head must be contiguous")
+    if first < 0 or first + batch > shape[0]:
+        raise ValueError(f"{what}: sequences {first}..{first + batch} of a 4-bit cache of {shape[0]}")
+    if written and shape[0] > 1 and stride[0] == 0:
+        raise ValueError(f"{what}: the 4-bit cache is written, its sequences must not share memory")
+
+
+def _check_int32(what, name, t, n):
+    if t.dtype != torch.int32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be {n} contiguous int32 values")
+
+
+def _check_rows(what, cache):
+    if cache.dim() != 5 or cache.shape[2] != 2:
+        raise ValueError(f"{what}: cache must be [batch, rows, 2, kv heads, head_dim]")
+    hk, d = cache.shape[3:]
+    if cache.stride()[2:] != (hk * d, d, 1):
+        raise ValueError(f"{what}: the values of a cache row must be contiguous")
+    return hk, d
+
+
+def quantize_cache_q4(cache, counts, cache_q4, starts=None, batch_offset=0):
+    """Rows [0, counts[b]) of cache[b] ([B, rows, 2, hkv, d]) become the records at positions
+    starts[b] + i (0 + i when starts is None) of cache_q4[batch_offset + b]; counts and starts are
+    int32 on the device. Returns cache_q4. Rows outside either buffer are skipped and reported in
+    the device error word (2)."""
+    hk, d = _check_rows("quantize_cache_q4", cache)
+    B = cache.shape[0]
+    _check_q4("quantize_cache_q4", cache_q4, hk, d, batch_offset, B, written=True)
+    _check_int32("quantize_cache_q4", "counts", counts, B)
+    if starts is not None:
+        _check_int32("quantize_cache_q4", "starts", starts, B)
+    dev = _device_of(cache, counts, cache_q4, starts)
+    if cache.numel() == 0:
+        return cache_q4
+    _call(dev, "hx_quantize_cache_q4", cache.data_ptr(), cache.stride(0), cache.stride(1),
+          cache.shape[1], _p(starts), counts.data_ptr(), B, hk, d, cache_q4.data_ptr(),
+          cache_q4.stride(0), cache_q4.stride(1), batch_offset, cache_q4.shape[2], _code(cache))
+    _count(1)
+    return cache_q4
+
+
+def dequantize_cache_q4(cache_q4, counts, cache, starts=None, batch_offset=0):
+    """The way back: records [starts[b], starts[b] + counts[b]) of cache_q4[batch_offset + b] as
+    rows [0, counts[b]) of cache[b] ([B, rows, 2, hkv, d]). Returns cache."""
+    hk, d = _check_rows("dequantize_cache_q4", cache)
+    B = cache.shape[0]
+    if B > 1 and cache.stride(0) == 0 or cache.shape[1] > 1 and cache.stride(1) == 0:
+        raise ValueError("dequantize_cache_q4: cache is written, its rows must not share memory")
+    _check_q4("dequantize_cache_q4", cache_q4, hk, d, batch_offset, B)
+    _check_int32("dequantize_cache_q4", "counts", counts, B)
+    if starts is not None:
+        _check_int32("dequantize_cache_q4", "starts", starts, B)
+    dev = _device_of(cache, counts, cache_q4, starts)
+    if cache.numel() == 0:
+        return cache
+    _call(dev, "hx_dequantize_cache_q4", cache_q4.data_ptr(), cache_q4.stride(0),
+          cache_q4.stride(1), batch_offset, cache_q4.shape[2], _p(starts), counts.data_ptr(), B, hk,
+          d, cache.data_ptr(), cache.stride(0), cache.stride(1), cache.shape[1], _code(cache))
+    _count(1)
+    return cache
+
+
+def rotary_cache_write_q4(qkv, batch, seqlen, n_heads, n_heads_kv, head_dim, pos_start, cos, sin,
+                          cache_q4, q_out=None, batch_offset=0, interleaved=True):
+    """rotary_cache_write into a 4-bit cache: rotates q/k of the packed qkv and writes k/v as the
+    records at positions pos_start[b] + s of cache_q4[batch_offset + b]. Returns q [batch, seqlen,
+    n_heads, head_dim]."""
+    what = "rotary_cache_write_q4"
+    _check_q4(what, cache_q4, n_heads_kv, head_dim, batch_offset, batch, written=True)
+    _check_int32(what, "pos_start", pos_start, batch)
+    if qkv.numel() != batch * seqlen * (n_heads + 2 * n_heads_kv) * head_dim or not qkv.is_contiguous():
+        raise ValueError(f"{what}: qkv must be contiguous [batch, seqlen, (n_heads + 2 n_heads_kv) * head_dim]")
+    for t in (cos, sin):
+        if t.dtype != qkv.dtype or t.shape != cos.shape or t.shape[-1] * 2 != head_dim or not t.is_contiguous():
+            raise ValueError(f"{what}: cos and sin must be contiguous [positions, head_dim / 2] in qkv's dtype")
+    dev = _device_of(qkv, cache_q4, pos_start, cos, sin, q_out)
+    if q_out is None:
+        q_out = torch.empty(batch, seqlen, n_heads, head_dim, dtype=qkv.dtype, device=qkv.device)
+    elif (q_out.numel() != batch * seqlen * n_heads * head_dim or q_out.dtype != qkv.dtype
+          or not q_out.is_contiguous()):
+        raise ValueError(f"{what}: q_out must be contiguous [batch, seqlen, n_heads, head_dim] in qkv's dtype")
+    if qkv.numel() == 0:
+        return q_out
+    _call(dev, "hx_rotary_cache_write_q4", qkv.data_ptr(), batch, seqlen, n_heads, n_heads_kv,
+          head_dim, pos_start.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+          1 if interleaved else 0, q_out.data_ptr(), cache_q4.data_ptr(), cache_q4.stride(0),
+          cache_q4.stride(1), batch_offset, cache_q4.shape[2], _code(qkv))
+    _count(1)
+    return q_out
+
+
+def decode_attention_q4(q, cache_q4, seqlens, n_heads_kv, max_seqlen, softmax_scale, out=None):
+    """decode_attention over a 4-bit cache: q [B, hq, d] against the first seqlens[b] records of
+    cache_q4[b] (seqlens int32 on device, each at most max_seqlen; 0 gives zeros)."""
+    what = "decode_attention_q4"
+    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+        raise ValueError(f"{what}: q must be [batch, n_heads, head_dim] with contiguous heads")
+    B, hq, d = q.shape
+    _check_q4(what, cache_q4, n_heads_kv, d, 0, B)
+    _check_int32(what, "seqlens", seqlens, B)
+    if not 0 <= max_seqlen <= cache_q4.shape[2]:
+        raise ValueError(f"{what}: max_seqlen {max_seqlen} of a 4-bit cache of {cache_q4.shape[2]} positions")
+    dev = _device_of(q, cache_q4, seqlens, out)
+    if out is None:
+        out = torch.empty(B, hq, d, dtype=q.dtype, device=q.device)
+    elif out.numel() != q.numel() or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be contiguous [batch, n_heads, head_dim] in q's dtype")
+    if B == 0:
+        return out
+    nbytes = decode_q4_workspace_bytes(B, hq, n_heads_kv, d, max_seqlen)
+    # A buffer of its own for every call: calls on several streams, and graphs, do not share it.
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _call(dev, "hx_decode_attention_q4", q.data_ptr(), q.stride(0), cache_q4.data_ptr(),
+          cache_q4.stride(0), cache_q4.stride(1), seqlens.data_ptr(), B, hq, n_heads_kv, d,
+          max_seqlen, float(softmax_scale), out.data_ptr(), _p(ws), nbytes, _code(q))
+    _count(2 if nbytes else 1)
+    return out
+
+
+def decode_q4_workspace_bytes(batch, n_heads, n_heads_kv, head_dim, max_seqlen) -> int:
+    return _L().hx_decode_attention_q4_workspace(batch, n_heads, n_heads_kv, head_dim, max_seqlen)
+
+
+# ----------------------------------------------------------------------------- 4-bit weights
+def gemm_q4(a, w_q4, scales, epilogue=HX_EPI_NONE, residual=None, out=None):
+    """gemm with a 4-bit weight for decode batches: out = a @ w.T with an epilogue, a [M, K] (M <= 64),
+    w_q4 uint8 [N, K / 2] and scales [N, K / group] in a's dtype as checkpoint.quantize_weight_q4
+    makes them (w = scale * (code - 8), group 32, 64 or 128)."""
+    what = "gemm_q4"
+    if a.dim() != 2 or w_q4.dim() != 2 or scales.dim() != 2 or a.stride(1) != 1:
+        raise ValueError(f"{what}: a, w_q4 and scales must be matrices, the rows of a contiguous")
+    M, K = a.shape
+    N = w_q4.shape[0]
+    if w_q4.dtype != torch.uint8 or w_q4.shape[1] * 2 != K or not w_q4.is_contiguous():
+        raise ValueError(f"{what}: w_q4 must be contiguous uint8 [N, K / 2]: got {tuple(w_q4.shape)} for K = {K}")
+    if (scales.dtype != a.dtype or scales.shape[0] != N or not scales.is_contiguous()
+            or scales.shape[1] == 0 or K % scales.shape[1]):
+        raise ValueError(f"{what}: scales must be contiguous [N, K / group] in a's dtype")
+    cols = N // 2 if epilogue == HX_EPI_SWIGLU else N
+    if (residual is None) != (epilogue != HX_EPI_RESIDUAL):
+        raise ValueError(f"{what}: a residual goes with HX_EPI_RESIDUAL and only with it")
+    for t in (residual, out):
+        if t is not None and (tuple(t.shape) != (M, cols) or t.dtype != a.dtype or t.stride(1) != 1):
+            raise ValueError(f"{what}: residual and out must be [M, {cols}] in a's dtype with contiguous rows")
+    if out is not None and M > 1 and out.stride(0) < cols:
+        raise ValueError(f"{what}: the rows of out must not share memory")
+    dev = _device_of(a, w_q4, scales, residual, out)
+    if out is None:
+        out = torch.empty(M, cols, dtype=a.dtype, device=a.device)
+    if M == 0:
+        return out
+    _call(dev, "hx_gemm_q4", a.data_ptr(), w_q4.data_ptr(), scales.data_ptr(), out.data_ptr(), M, N,
+          K, K // scales.shape[1], a.stride(0) if M > 1 else max(K, a.stride(0)),
+          out.stride(0) if M > 1 else cols, epilogue, _p(residual),
+          0 if residual is None else residual.stride(0) if M > 1 else cols, _code(a))
+    _count(1)
+    return out
+
+
 # ----------------------------------------------------------------------------- sampling
 def argmax(logits, out=None):
     _require_cuda(logits)
@@ -293,6 +499,40 @@ def argmax(logits, out=None):
                          _stream()), "hx_argmax")
     _count(1)
     return out
+
+
+TokenLogprobs = namedtuple("TokenLogprobs", ["logprobs", "entropy", "top_logprobs", "top_tokens"])
+
+
+def token_logprobs(logits, tokens=None, top_k=0, entropy=False) -> TokenLogprobs:
+    """What a row of logits [rows, vocab] says of its tokens, in f32: logprobs [rows] of the given
+    tokens (int64 [rows]; None without them; NaN for a token outside the vocabulary), the
+    distribution's entropy in nats [rows] (None unless asked for), and the top_k <= 32 most likely
+    tokens with their log probabilities [rows, top_k] (None for 0), equal logits by the lower index.
+    Masked (-inf) logits have probability 0; a row with a NaN or +inf, or of -inf alone, gives NaN."""
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("token_logprobs: logits must be [rows, vocab] with contiguous rows")
+    rows, cols = logits.shape
+    if tokens is not None and (tokens.dtype != torch.long or tokens.numel() != rows
+                               or not tokens.is_contiguous()):
+        raise ValueError(f"token_logprobs: tokens must be {rows} contiguous int64 values")
+    if tokens is None and not entropy and top_k == 0:
+        raise ValueError("token_logprobs: nothing is asked for")
+    dev = _device_of(logits, tokens)
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    logp = None if tokens is None else torch.empty(rows, **f32)
+    ent = torch.empty(rows, **f32) if entropy else None
+    top = ids = None
+    if top_k > 0:
+        top = torch.empty(rows, top_k, **f32)
+        ids = torch.empty(rows, top_k, dtype=torch.long, device=logits.device)
+    if rows == 0:
+        return TokenLogprobs(logp, ent, top, ids)
+    _call(dev, "hx_token_logprobs", logits.data_ptr(), rows, cols,
+          logits.stride(0) if rows > 1 else max(cols, logits.stride(0)), _p(tokens), top_k, _p(logp),
+          _p(ent), _p(top), _p(ids), _code(logits))
+    _count(1)
+    return TokenLogprobs(logp, ent, top, ids)
 
 
 # ----------------------------------------------------------------------------- KV handoff

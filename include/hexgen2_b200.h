@@ -220,11 +220,89 @@ int hx_decode_attention_noalloc(const void* q, const void* cache, int64_t cache_
                                 int64_t head_dim, int64_t max_seqlen_k, float softmax_scale,
                                 void* out, int dtype, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit KV cache */
+/* The KV cache held in 4 bits (no counterpart in the reference): cache_q4 is
+ * [batch, n_heads_kv, max_seq, head_dim + 16] bytes, one record per position and KV head:
+ * head_dim/2 bytes of K codes (element 2j in the low nibble of byte j, 2j + 1 in the high one),
+ * head_dim/2 bytes of V codes, then k_scale, k_min, v_scale, v_min in f32. A row x is stored as
+ * (f32, one IEEE operation each) lo = min x, R = max x - lo, scale = R / 15, code =
+ * min(15, rint((x - lo) * (15 / R))) and reads back as lo + scale * code. R < 2^-100 gives scale 0
+ * and codes 0; a row with a value that is not finite (or R not finite) reads back as NaN.
+ * q4_batch_stride and q4_head_stride are in bytes, multiples of 16; the records of a head are
+ * contiguous. Each record is a multiple of 16 bytes, so hx_kv_pack / hx_kv_unpack move the live
+ * records of a layer as n_heads_kv outer slices of rows of head_dim + 16 bytes. head_dim 32, 64
+ * or 128, f32/f16/bf16 rows.
+ *
+ * hx_quantize_cache_q4: rows [0, counts[b]) of cache[b] ([batch, cache_rows, 2, n_heads_kv,
+ * head_dim], strides in elements, rows 16-byte aligned) become the records at positions
+ * starts[b] + i (starts NULL: 0) of cache_q4[q4_batch_offset + b]. hx_dequantize_cache_q4 is the
+ * way back. starts and counts are device int32. Rows that either buffer does not hold (and
+ * negative starts or counts) are left alone and set the device error word to 2. No record or row
+ * outside the ranges is written. */
+int hx_quantize_cache_q4(const void* cache, int64_t cache_batch_stride, int64_t cache_seq_stride,
+                         int64_t cache_rows, const int32_t* starts, const int32_t* counts,
+                         int64_t batch, int64_t n_heads_kv, int64_t head_dim, void* cache_q4,
+                         int64_t q4_batch_stride, int64_t q4_head_stride, int64_t q4_batch_offset,
+                         int64_t q4_max_seq, int dtype, void* stream);
+int hx_dequantize_cache_q4(const void* cache_q4, int64_t q4_batch_stride, int64_t q4_head_stride,
+                           int64_t q4_batch_offset, int64_t q4_max_seq, const int32_t* starts,
+                           const int32_t* counts, int64_t batch, int64_t n_heads_kv,
+                           int64_t head_dim, void* cache, int64_t cache_batch_stride,
+                           int64_t cache_seq_stride, int64_t cache_rows, int dtype, void* stream);
+/* hx_rotary_cache_write into a 4-bit cache: q rotated to q_out, k (rotated, rounded to dtype) and v
+ * as records at position pos_start[b] + s of cache_q4[q4_batch_offset + b]. The records are those
+ * hx_quantize_cache_q4 makes of the rows hx_rotary_cache_write writes. A token whose position
+ * lies outside the cache or the tables is skipped and sets the device error word to 2. qkv and
+ * q_out 16-byte aligned. */
+int hx_rotary_cache_write_q4(const void* qkv, int64_t batch, int64_t seqlen, int64_t n_heads,
+                             int64_t n_heads_kv, int64_t head_dim, const int32_t* pos_start,
+                             const void* cos_table, const void* sin_table, int64_t table_rows,
+                             int interleaved, void* q_out, void* cache_q4, int64_t q4_batch_stride,
+                             int64_t q4_head_stride, int64_t q4_batch_offset, int64_t q4_max_seq,
+                             int dtype, void* stream);
+/* hx_decode_attention over a 4-bit cache: q [batch, n_heads, head_dim] (rows of sequences at
+ * q_batch_stride elements), sequence b attends to the first seqlens_k[b] records of each KV head
+ * of cache_q4[b]; out [batch, n_heads, head_dim] contiguous. Any number of query heads per KV
+ * head. A sequence of length 0 gives zeros; a length above max_seqlen_k (or below 0) is cut to it
+ * and sets the device error word to 2. workspace: hx_decode_attention_q4_workspace() bytes, not
+ * shared by calls that may overlap. */
+int hx_decode_attention_q4(const void* q, int64_t q_batch_stride, const void* cache_q4,
+                           int64_t q4_batch_stride, int64_t q4_head_stride,
+                           const int32_t* seqlens_k, int64_t batch, int64_t n_heads,
+                           int64_t n_heads_kv, int64_t head_dim, int64_t max_seqlen_k,
+                           float softmax_scale, void* out, void* workspace,
+                           size_t workspace_bytes, int dtype, void* stream);
+size_t hx_decode_attention_q4_workspace(int64_t batch, int64_t n_heads, int64_t n_heads_kv,
+                                        int64_t head_dim, int64_t max_seqlen_k);
+
+/* ---------------------------------------------------------------- 4-bit weights */
+/* c[m, n] = sum over groups g of scales[n, g] * sum over k in g of a[m, k] * (code[n, k] - 8), for
+ * decode batches (m <= 64), f32 accumulation, one rounding at the end. w: [n, k/2] bytes
+ * contiguous (element 2j in the low nibble of byte j), scales: [n, k/group] contiguous in dtype,
+ * group 32, 64 or 128 dividing k. Epilogues NONE, RESIDUAL (+ residual[m, n]) and SWIGLU (rows of
+ * w interleaved [up16|gate16], c has n/2 columns), as hx_gemm's but in f32 up to the one rounding.
+ * a 16-byte aligned with lda a multiple of 16 bytes; w 16-byte aligned. residual may be c. No
+ * workspace. No counterpart in the reference. */
+int hx_gemm_q4(const void* a, const void* w, const void* scales, void* c, int64_t m, int64_t n,
+               int64_t k, int64_t group, int64_t lda, int64_t ldc, int epilogue,
+               const void* residual, int64_t ld_residual, int dtype, void* stream);
+
 /* ---------------------------------------------------------------- sampling */
 /* out_idx[r] = first index of the maximum of logits[r, 0:cols] (torch.argmax semantics).
  * Replaces logits.argmax(-1) at hexgen2/model.py:82 and :117. */
 int hx_argmax(const void* logits, int64_t rows, int64_t cols, int64_t ld, int64_t* out_idx,
               int dtype, void* stream);
+
+/* Log probabilities of given tokens, entropy (nats) and the most likely tokens of each row of
+ * logits [rows, cols] (row stride ld): logprobs[r] = log softmax(logits[r])[tokens[r]] (NaN for a
+ * token outside [0, cols)), entropy[r], and top_logprobs / top_tokens [rows, top_k] in falling
+ * order, equal logits by the lower index (NaN first). f32 arithmetic and outputs. top_k <= 32 and
+ * <= cols. logprobs (with tokens), entropy and, for top_k 0, the top list may be NULL. -inf logits
+ * have probability 0; a row with a NaN or +inf, or of -inf alone, gives NaN, as torch.log_softmax.
+ * No counterpart in the reference. */
+int hx_token_logprobs(const void* logits, int64_t rows, int64_t cols, int64_t ld,
+                      const int64_t* tokens, int64_t top_k, float* logprobs, float* entropy,
+                      float* top_logprobs, int64_t* top_tokens, int dtype, void* stream);
 
 /* ---------------------------------------------------------------- KV handoff */
 /* Gather-pack of live cache rows for n_req requests into one contiguous buffer.
