@@ -166,6 +166,352 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
   }
 }
 
+// ------------------------------------------------------------------------------------------
+// Tensor-core kernel (f16/bf16). The codes are at most 15, so a 16-bit float holds them exactly:
+// S = K codes . q^T and O^T = V codes^T . P'^T (P' = p * v_scale) run on mma.m16n8k16 with f32
+// sums, the 16 rows of A being positions (S) or output elements (O) and its 8 columns query heads.
+//   - A nibble becomes a float by OR-ing it into the mantissa of a constant: 128 + code in bf16,
+//     16 + code in f16. The constant's share of S is bias * sum(q), of O bias * sum(P'); both are
+//     subtracted with the scales (f32, 2^-24 of 17 times the codes' own share at most).
+//   - The two nibbles 16 bits apart in a word make one operand register. The order of the D
+//     elements in S and of the output elements in O is free, so each lane takes the words it
+//     can read with one wide load: for S 1/4 of a position's K codes, for O 1/8 of a position's V codes.
+//   - P' (any size: v_scale is not bounded) goes in as the sum of two bf16, 2^-17 relative.
+//   - S comes out position-major; movmatrix turns it into the B operand of O.
+// Each warp streams 32-position tiles through a ring of its own (bulk copies by its lane 0, one
+// mbarrier per stage): no block barrier until the warps' partials are added up at the end.
+// ------------------------------------------------------------------------------------------
+constexpr int kTile = 32;    // positions per stage
+constexpr int kStages = 4;
+
+template <typename T> struct Codes;
+template <> struct Codes<__nv_bfloat16> {
+  static constexpr float kBias = 128.f;
+  template <int E> static HX_DEVICE uint32_t pair(uint32_t w) {  // nibbles E and E + 4
+    return ((w >> (4 * E)) & 0x000f000fu) | 0x43004300u;
+  }
+};
+template <> struct Codes<__half> {
+  static constexpr float kBias = 16.f;
+  template <int E> static HX_DEVICE uint32_t pair(uint32_t w) {
+    const uint32_t at = E == 0 ? w << 6 : E == 1 ? w << 2 : E == 2 ? w >> 2 : w >> 6;
+    return (at & 0x03c003c0u) | 0x4c004c00u;
+  }
+};
+
+template <typename T>
+HX_DEVICE void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Transpose of the 8x8 16-bit matrix that a warp holds one row pair per lane.
+HX_DEVICE uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+HX_DEVICE void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+template <int D, int NT>
+struct McSmem {
+  static constexpr int kRing = kWarps * kStages * kTile * (D + 16);
+  static constexpr int kMerge = kWarps * NT * 8 * D * 4;
+  static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge);
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
+  constexpr int kRec = D + 16, W = D / 32, OT = D / 16;
+  constexpr float kBias = Codes<T>::kBias, kBiasV = Codes<__nv_bfloat16>::kBias;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[kWarps][kStages];
+  __shared__ float sm_m[kWarps][NT * 8], sm_l[kWarps][NT * 8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
+  pdl_wait();
+  pdl_trigger();
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int hk = blockIdx.y / a.q_chunks, h0 = hk * a.group + (blockIdx.y % a.q_chunks) * (NT * 8);
+  const int nq = min(NT * 8, (hk + 1) * a.group - h0);
+  const int len = live_length(a.seqlens, b, a.max_len);
+  const int start = split * a.chunk, end = min(start + a.chunk, len);
+  T* out = (T*)a.out + ((int64_t)b * a.n_heads + h0) * D;
+  if (start >= end) {
+    if (a.splits == 1)
+      for (int i = tid; i < nq * D; i += kThreads) out[i] = DT<T>::from_f(0.f);
+    return;
+  }
+  const uint8_t* recs = a.q4 + (int64_t)b * a.qbs + (int64_t)hk * a.qhs;
+  uint8_t* ring = smem + warp * (kStages * kTile * kRec);
+  const int first = start + warp * kTile;
+  const int n_tiles = first < end ? (end - first + kWarps * kTile - 1) / (kWarps * kTile) : 0;
+  // Lane 0: tile i (positions first + 128 i ...) into stage i % kStages; never past the live end.
+  auto load = [&](int i) {
+    const int at = first + i * (kWarps * kTile);
+    const uint32_t bytes = (uint32_t)min(kTile, end - at) * kRec;
+    uint64_t* bar = &full[warp][i % kStages];
+    mbar_arrive_expect_tx(bar, bytes);
+    bulk_load(ring + (i % kStages) * (kTile * kRec), recs + (int64_t)at * kRec, bytes, bar);
+  };
+  if (lane == 0)
+    for (int i = 0; i < min(n_tiles, kStages); ++i) load(i);
+
+  // q as B operands: lane (g, t) holds head g's elements of K words [W t, W t + W).
+  uint32_t qf[NT][2 * W][2];
+  float qsum[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int h = nt * 8 + g;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (h < nq)
+        raw = *reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)b * a.q_stride +
+                                              (int64_t)(h0 + h) * D + (t * W + w) * 8);
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += DT<T>::to_f(e[i]);
+      // elements (0,4), (1,5) and (2,6), (3,7): the order pair<E> gives the codes
+      qf[nt][2 * w][0] = __byte_perm(raw.x, raw.z, 0x5410);
+      qf[nt][2 * w][1] = __byte_perm(raw.x, raw.z, 0x7632);
+      qf[nt][2 * w + 1][0] = __byte_perm(raw.y, raw.w, 0x5410);
+      qf[nt][2 * w + 1][1] = __byte_perm(raw.y, raw.w, 0x7632);
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    qsum[nt][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+    qsum[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+  }
+
+  // Per lane, for query heads 2t and 2t + 1 of each tile of eight: running maximum (the same in all
+  // lanes of equal t), this lane's share of the sums, and the output elements of its rows.
+  float m[NT][2], l[NT][2], z[NT][2], o[NT][OT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    m[nt][0] = m[nt][1] = -INFINITY;
+    l[nt][0] = l[nt][1] = z[nt][0] = z[nt][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < OT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
+  }
+
+  int done = 0;
+  for (; done < n_tiles; ++done) {
+    const int stage = done % kStages;
+    if (!mbar_wait_warp(&full[warp][stage], (done / kStages) & 1)) break;
+    const uint8_t* tile = ring + stage * (kTile * kRec);
+    const int n = min(kTile, end - (first + done * (kWarps * kTile)));
+    float s[2][NT][4];
+    float4 meta[2][2];
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      const uint8_t* r0 = tile + (sub * 16 + g) * kRec;
+      const uint8_t* r1 = r0 + 8 * kRec;
+      uint32_t k0[W], k1[W];
+      if constexpr (W == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(r0 + 16 * t), y = *reinterpret_cast<const uint4*>(r1 + 16 * t);
+        k0[0] = x.x, k0[1] = x.y, k0[2] = x.z, k0[3] = x.w;
+        k1[0] = y.x, k1[1] = y.y, k1[2] = y.z, k1[3] = y.w;
+      } else if constexpr (W == 2) {
+        const uint2 x = *reinterpret_cast<const uint2*>(r0 + 8 * t), y = *reinterpret_cast<const uint2*>(r1 + 8 * t);
+        k0[0] = x.x, k0[1] = x.y, k1[0] = y.x, k1[1] = y.y;
+      } else {
+        k0[0] = *reinterpret_cast<const uint32_t*>(r0 + 4 * t);
+        k1[0] = *reinterpret_cast<const uint32_t*>(r1 + 4 * t);
+      }
+      meta[sub][0] = *reinterpret_cast<const float4*>(r0 + D);
+      meta[sub][1] = *reinterpret_cast<const float4*>(r1 + D);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[sub][nt][j] = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const uint32_t lo[4] = {Codes<T>::template pair<0>(k0[w]), Codes<T>::template pair<0>(k1[w]),
+                                Codes<T>::template pair<1>(k0[w]), Codes<T>::template pair<1>(k1[w])};
+        const uint32_t hi[4] = {Codes<T>::template pair<2>(k0[w]), Codes<T>::template pair<2>(k1[w]),
+                                Codes<T>::template pair<3>(k0[w]), Codes<T>::template pair<3>(k1[w])};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<T>(s[sub][nt], lo, qf[nt][2 * w][0], qf[nt][2 * w][1]);
+          mma16816<T>(s[sub][nt], hi, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+        }
+      }
+    }
+    // Scores in base 2, and the tile's maximum per query head.
+    float top[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float ks = meta[sub][r].x * a.scale_log2;
+        const float km = meta[sub][r].y * a.scale_log2 - kBias * ks;
+        const bool live = sub * 16 + r * 8 + g < n;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float& x = s[sub][nt][2 * r + j];
+            x = live ? fmaf(ks, x, km * qsum[nt][j]) : -INFINITY;
+            top[nt][j] = fmaxf(top[nt][j], x);
+          }
+      }
+    bool grows = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1)
+          top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], x));
+        grows |= top[nt][j] > m[nt][j] + 8.f;
+      }
+    // The reference m follows the maximum only when it is left behind by more than 2^8: until then p
+    // stays below 2^8, which f32 sums and the final quotient do not notice.
+    if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float next = fmaxf(m[nt][j], top[nt][j]);
+          const float f = ex2_approx(m[nt][j] - next);
+          m[nt][j] = next;
+          l[nt][j] *= f;
+          z[nt][j] *= f;
+#pragma unroll
+          for (int i = 0; i < OT; ++i) o[nt][i][j] *= f, o[nt][i][2 + j] *= f;
+        }
+    }
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const bool live = sub * 16 + r * 8 + g < n;
+          float hi[2], lo[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float p = live ? ex2_approx(s[sub][nt][2 * r + j] - m[nt][j]) : 0.f;
+            const float pv = live ? p * meta[sub][r].z : 0.f;  // stale scales may be NaN
+            hi[j] = round_to<__nv_bfloat16>(pv);
+            lo[j] = round_to<__nv_bfloat16>(pv - hi[j]);
+            l[nt][j] += p;
+            z[nt][j] += (live ? p * meta[sub][r].w : 0.f) - kBiasV * (hi[j] + lo[j]);
+          }
+          bh[nt][r] = transpose8x8(pack2<__nv_bfloat16>(hi[0], hi[1]));
+          bl[nt][r] = transpose8x8(pack2<__nv_bfloat16>(lo[0], lo[1]));
+        }
+      // V codes of positions 2t, 2t + 1, 2t + 8, 2t + 9: lane (g, t) takes bytes [D/16 g, D/16 (g + 1)).
+      const uint8_t* v = tile + (sub * 16 + 2 * t) * kRec + D / 2 + (D / 16) * g;
+      constexpr int VW = D >= 64 ? D / 64 : 1;
+      uint32_t vw[4][VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* at = v + ((i & 1) + 8 * (i >> 1)) * kRec;
+        if constexpr (D == 128) {
+          const uint2 x = *reinterpret_cast<const uint2*>(at);
+          vw[i][0] = x.x, vw[i][1] = x.y;
+        } else if constexpr (D == 64) {
+          vw[i][0] = *reinterpret_cast<const uint32_t*>(at);
+        } else {
+          vw[i][0] = *reinterpret_cast<const uint16_t*>(at);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < OT; ++i) {
+        const uint32_t sel = (i % 4) * 0x0011u + (4 + i % 4) * 0x1100u;
+        const uint32_t x = __byte_perm(vw[0][i / 4], vw[1][i / 4], sel);
+        const uint32_t y = __byte_perm(vw[2][i / 4], vw[3][i / 4], sel);
+        const uint32_t av[4] = {(x & 0x000f000fu) | 0x43004300u, ((x >> 4) & 0x000f000fu) | 0x43004300u,
+                                (y & 0x000f000fu) | 0x43004300u, ((y >> 4) & 0x000f000fu) | 0x43004300u};
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          mma16816<__nv_bfloat16>(o[nt][i], av, bh[nt][0], bh[nt][1]);
+          mma16816<__nv_bfloat16>(o[nt][i], av, bl[nt][0], bl[nt][1]);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0 && done + kStages < n_tiles) load(done + kStages);
+  }
+  if (done < n_tiles) {  // a wait gave up: let the copies in flight land before the ring is reused
+    for (int i = done; i < min(n_tiles, done + kStages); ++i)
+      mbar_wait_drain(&full[warp][i % kStages], (i / kStages) & 1);
+  }
+  // Lane shares to warp sums, then the warps' partials through shared memory (the rings are idle).
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) {
+        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], x);
+        z[nt][j] += __shfl_xor_sync(0xffffffffu, z[nt][j], x);
+      }
+      if (g == 0) sm_m[warp][nt * 8 + 2 * t + j] = m[nt][j], sm_l[warp][nt * 8 + 2 * t + j] = l[nt][j];
+    }
+  __syncthreads();
+  float* sm_o = reinterpret_cast<float*>(smem);  // [kWarps][NT * 8][D]
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < OT; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<float2*>(sm_o + (warp * NT * 8 + nt * 8 + 2 * t + j) * D + (D / 8) * g + 2 * i) =
+            make_float2(o[nt][i][j] + z[nt][j], o[nt][i][2 + j] + z[nt][j]);
+  __syncthreads();
+  for (int i = tid; i < nq * D; i += kThreads) {
+    const int q = i / D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][q]);
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (start + w * kTile >= end) continue;  // this warp had no positions
+      const float f = exp2f(sm_m[w][q] - M);
+      L += f * sm_l[w][q];
+      O += f * sm_o[(w * NT * 8) * D + i];
+    }
+    if (a.splits == 1) {
+      out[i] = DT<T>::from_f(O / L);
+    } else {
+      const int64_t slot = ((int64_t)b * a.n_heads + h0 + q) * a.splits + split;
+      a.ws_o[slot * D + i % D] = O;
+      if (i % D == 0) a.ws_ml[2 * slot] = M, a.ws_ml[2 * slot + 1] = L;
+    }
+  }
+}
+
 // out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s over the splits that hold keys: one CTA per
 // (sequence, query head), one thread per output element.
 template <typename T, int D>
@@ -201,11 +547,29 @@ Plan plan(int64_t batch, int64_t n_heads, int64_t n_heads_kv, int64_t max_len) {
   return {(int)(per * 128), (int)((steps + per - 1) / per)};
 }
 
+template <typename T, int D, int NT>
+int launch_mma(Args& a, int64_t batch, int64_t n_heads_kv, cudaStream_t stream) {
+  a.q_chunks = ceil_div(a.group, NT * 8);
+  constexpr int smem = McSmem<D, NT>::kBytes;
+  auto kern = decode_q4_mma_kernel<T, D, NT>;
+  if (smem > 48 * 1024)
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const dim3 grid((unsigned)a.splits, (unsigned)(n_heads_kv * a.q_chunks), (unsigned)batch);
+  return hx::cuda_status(launch_ex(kern, grid, dim3(kThreads), smem, stream, 1, a),
+                         "decode_q4_mma_kernel launch");
+}
+
 template <typename T, int D>
 int launch(Args a, int64_t batch, int64_t n_heads_kv, cudaStream_t stream) {
-  const dim3 grid((unsigned)a.splits, (unsigned)(n_heads_kv * a.q_chunks), (unsigned)batch);
-  int s = hx::cuda_status(launch_ex(decode_q4_kernel<T, D>, grid, dim3(kThreads), 0, stream, 1, a),
-                          "decode_q4_kernel launch");
+  int s;
+  if constexpr (sizeof(T) == 2) {
+    s = a.group > 8 ? launch_mma<T, D, 2>(a, batch, n_heads_kv, stream)
+                    : launch_mma<T, D, 1>(a, batch, n_heads_kv, stream);
+  } else {
+    const dim3 grid((unsigned)a.splits, (unsigned)(n_heads_kv * a.q_chunks), (unsigned)batch);
+    s = hx::cuda_status(launch_ex(decode_q4_kernel<T, D>, grid, dim3(kThreads), 0, stream, 1, a),
+                        "decode_q4_kernel launch");
+  }
   if (s || a.splits == 1) return s;
   return hx::cuda_status(launch_ex(decode_q4_merge_kernel<T, D>, dim3((unsigned)(batch * a.n_heads)),
                                    dim3(D), 0, stream, 1, a),
