@@ -167,58 +167,49 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------------------------------
-// Tensor-core kernel (f16/bf16). The codes are at most 15, so a 16-bit float holds them exactly:
-// S = K codes . q^T and O^T = V codes^T . P'^T (P' = p * v_scale) run on mma.m16n8k16 with f32
-// sums, the 16 rows of A being positions (S) or output elements (O) and its 8 columns query heads.
-//   - A nibble becomes a float by OR-ing it into the mantissa of a constant: 128 + code in bf16,
-//     16 + code in f16. The constant's share of S is bias * sum(q), of O bias * sum(P'); both are
-//     subtracted with the scales (f32, 2^-24 of 17 times the codes' own share at most).
-//   - The two nibbles 16 bits apart in a word make one operand register. The order of the D
-//     elements in S and of the output elements in O is free, so each lane takes the words it
-//     can read with one wide load: for S 1/4 of a position's K codes, for O 1/8 of a position's V codes.
-//   - P' (any size: v_scale is not bounded) goes in as the sum of two bf16, 2^-17 relative.
+// Tensor-core kernel (f16/bf16): S = K codes . q^T and O^T = V codes^T . P'^T with P' = p * v_scale, on
+// mma.m16n8k16 with f16 operands and f32 sums; the 16 rows of A are positions (S) or output elements
+// (O), its 8 columns query heads.
+//   - The bits of a code are an f16 as they stand: below 2^11 an f16's value is its bits times 2^-24
+//     (subnormals and the first binade). A masked word is an operand register: w & 0x000f000f
+//     holds codes * 2^-24, w & 0x00f000f0 codes * 2^-20; no bias, no conversion, nothing rounded.
+//     The tensor core takes subnormals as they are.
+//   - q goes in as f16 times a power of two of its own per head (max |q| in [2^9, 2^10), times 16
+//     where the codes are not): bf16 and f16 values down to 2^-24 of the head's largest are exact.
+//   - The order of the D elements in S and of the output elements in O is free, so each lane takes
+//     the words it can read with one wide load: for S 1/4 of a position's K codes, for O 1/8 of
+//     a position's V codes (bytes of two positions joined with one permute).
+//   - P' enters as f16, relative to the largest P' seen (the running reference r follows
+//     s + log2 v_scale, not s): 2^-12 of each value, 2^-25 * 2^-7 of the largest. For f16 outputs, whose
+//     half step is no coarser than that, P' is the sum of two f16.
 //   - S comes out position-major; movmatrix turns it into the B operand of O.
 // Each warp streams 32-position tiles through a ring of its own (bulk copies by its lane 0, one
 // mbarrier per stage): no block barrier until the warps' partials are added up at the end.
+// NT tiles of eight columns; NJ = 1 puts at most four heads into the even columns, which halves the
+// softmax work per position.
 // ------------------------------------------------------------------------------------------
 constexpr int kTile = 32;    // positions per stage
 constexpr int kStages = 4;
 
-template <typename T> struct Codes;
-template <> struct Codes<__nv_bfloat16> {
-  static constexpr float kBias = 128.f;
-  template <int E> static HX_DEVICE uint32_t pair(uint32_t w) {  // nibbles E and E + 4
-    return ((w >> (4 * E)) & 0x000f000fu) | 0x43004300u;
-  }
-};
-template <> struct Codes<__half> {
-  static constexpr float kBias = 16.f;
-  template <int E> static HX_DEVICE uint32_t pair(uint32_t w) {
-    const uint32_t at = E == 0 ? w << 6 : E == 1 ? w << 2 : E == 2 ? w >> 2 : w >> 6;
-    return (at & 0x03c003c0u) | 0x4c004c00u;
-  }
-};
-
-template <typename T>
-HX_DEVICE void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                       const uint32_t (&b)[2]) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
 
 // Transpose of the 8x8 16-bit matrix that a warp holds one row pair per lane.
 HX_DEVICE uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+HX_DEVICE float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -237,13 +228,170 @@ struct McSmem {
   static constexpr int kBytes = (kRing > kMerge ? kRing : kMerge);
 };
 
-template <typename T, int D, int NT>
+// State of one warp's online softmax. Per lane, for columns 2t + j of each tile of eight: the
+// reference r (the same in all lanes of equal t), this lane's shares of sum p and sum p v_min, and
+// the output elements of its rows, even elements times 2^-24, odd ones times 2^-20.
+template <int D, int NT, int NJ>
+struct Softmax {
+  float r[NT][NJ], l[NT][NJ], z[NT][NJ], o[NT][D / 16][4];
+};
+
+constexpr float kFloor = -32.f;  // log2 of the smallest v_scale that the reference follows
+
+// One tile of n positions (kFull: n = kTile) in shared memory.
+template <typename T, int D, int NT, int NJ, bool kFull>
+HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const uint32_t (&qf)[NT][D / 16][2],
+                           const float (&qscale)[NT][NJ], const float (&qsum)[NT][NJ],
+                           Softmax<D, NT, NJ>& st) {
+  constexpr int kRec = D + 16, W = D / 32, OT = D / 16;
+  constexpr bool kTwo = std::is_same<T, __half>::value;  // P' as the sum of two f16
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  float s[2][NT][4];
+  float4 meta[2][2];
+#pragma unroll
+  for (int sub = 0; sub < 2; ++sub) {
+    const uint8_t* r0 = tile + (sub * 16 + g) * kRec;
+    const uint8_t* r1 = r0 + 8 * kRec;
+    uint32_t k0[W], k1[W];
+    if constexpr (W == 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(r0 + 16 * t), y = *reinterpret_cast<const uint4*>(r1 + 16 * t);
+      k0[0] = x.x, k0[1] = x.y, k0[2] = x.z, k0[3] = x.w;
+      k1[0] = y.x, k1[1] = y.y, k1[2] = y.z, k1[3] = y.w;
+    } else if constexpr (W == 2) {
+      const uint2 x = *reinterpret_cast<const uint2*>(r0 + 8 * t), y = *reinterpret_cast<const uint2*>(r1 + 8 * t);
+      k0[0] = x.x, k0[1] = x.y, k1[0] = y.x, k1[1] = y.y;
+    } else {
+      k0[0] = *reinterpret_cast<const uint32_t*>(r0 + 4 * t);
+      k1[0] = *reinterpret_cast<const uint32_t*>(r1 + 4 * t);
+    }
+    meta[sub][0] = *reinterpret_cast<const float4*>(r0 + D);
+    meta[sub][1] = *reinterpret_cast<const float4*>(r1 + D);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[sub][nt][j] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // elements (0,4), (1,5), then (2,6), (3,7) of the word
+        const uint32_t x = k0[w] >> (8 * h), y = k1[w] >> (8 * h);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma_f16(s[sub][nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u,
+                  qf[nt][2 * w + h]);
+      }
+  }
+  // Scores in base 2, and the tile's largest score + log2 v_scale per head.
+  float top[NT][NJ];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) top[nt][j] = -INFINITY;
+#pragma unroll
+  for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float ks = meta[sub][r].x * scale_log2, km = meta[sub][r].y * scale_log2;
+      const float lv = fmaxf(lg2_approx(meta[sub][r].z), kFloor);
+      const bool live = kFull || sub * 16 + r * 8 + g < n;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          float& x = s[sub][nt][2 * r + j];
+          x = fmaf(ks, x * qscale[nt][j], km * qsum[nt][j]);
+          if (!live) x = -INFINITY;
+          top[nt][j] = fmaxf(top[nt][j], x + lv);
+        }
+    }
+  bool grows = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1)
+        top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], x));
+      grows |= top[nt][j] > st.r[nt][j] + 15.f;
+    }
+  // The reference keeps P' below 2^15; it moves only when a tile would leave that range.
+  if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const float next = fmaxf(st.r[nt][j], top[nt][j] - 7.f);
+        const float f = ex2_approx(st.r[nt][j] - next);
+        st.r[nt][j] = next;
+        st.l[nt][j] *= f;
+        st.z[nt][j] *= f;
+#pragma unroll
+        for (int i = 0; i < OT; ++i) st.o[nt][i][j] *= f, st.o[nt][i][2 + j] *= f;
+      }
+  }
+#pragma unroll
+  for (int sub = 0; sub < 2; ++sub) {
+    uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const bool live = kFull || sub * 16 + r * 8 + g < n;  // stale scales may be NaN
+        float pv[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const float p = ex2_approx(s[sub][nt][2 * r + j] - st.r[nt][j]);
+          if (live) {
+            st.l[nt][j] += p;
+            st.z[nt][j] = fmaf(p, meta[sub][r].w, st.z[nt][j]);
+            pv[j] = p * meta[sub][r].z;
+          }
+        }
+        const uint32_t hi = pack2<__half>(pv[0], pv[1]);
+        bh[nt][r] = transpose8x8(hi);
+        if (kTwo) {
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+          bl[nt][r] = transpose8x8(pack2<__half>(pv[0] - back.x, pv[1] - back.y));
+        }
+      }
+    // V codes of positions 2t, 2t + 1, 2t + 8, 2t + 9: lane (g, t) takes bytes [D/16 g, D/16 (g + 1)).
+    const uint8_t* v = tile + (sub * 16 + 2 * t) * kRec + D / 2 + (D / 16) * g;
+    constexpr int VW = D >= 64 ? D / 64 : 1;
+    uint32_t vw[4][VW];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* at = v + ((i & 1) + 8 * (i >> 1)) * kRec;
+      if constexpr (D == 128) {
+        const uint2 x = *reinterpret_cast<const uint2*>(at);
+        vw[i][0] = x.x, vw[i][1] = x.y;
+      } else if constexpr (D == 64) {
+        vw[i][0] = *reinterpret_cast<const uint32_t*>(at);
+      } else {
+        vw[i][0] = *reinterpret_cast<const uint16_t*>(at);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < OT; ++i) {
+      const uint32_t sel = (i % 4) * 0x0011u + (4 + i % 4) * 0x1100u;
+      const uint32_t x = __byte_perm(vw[0][i / 4], vw[1][i / 4], sel);
+      const uint32_t y = __byte_perm(vw[2][i / 4], vw[3][i / 4], sel);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_f16(st.o[nt][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, bh[nt]);
+        if (kTwo)
+          mma_f16(st.o[nt][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, bl[nt]);
+      }
+    }
+  }
+}
+
+template <typename T, int D, int NT, int NJ>
 __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
   constexpr int kRec = D + 16, W = D / 32, OT = D / 16;
-  constexpr float kBias = Codes<T>::kBias, kBiasV = Codes<__nv_bfloat16>::kBias;
+  constexpr int kHeads = NT * 4 * NJ;  // head h sits in column h (NJ = 2) or 2h (NJ = 1)
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][kStages];
-  __shared__ float sm_m[kWarps][NT * 8], sm_l[kWarps][NT * 8];
+  __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(&full[warp][s], 1);
@@ -253,8 +401,8 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
   pdl_wait();
   pdl_trigger();
   const int split = blockIdx.x, b = blockIdx.z;
-  const int hk = blockIdx.y / a.q_chunks, h0 = hk * a.group + (blockIdx.y % a.q_chunks) * (NT * 8);
-  const int nq = min(NT * 8, (hk + 1) * a.group - h0);
+  const int hk = blockIdx.y / a.q_chunks, h0 = hk * a.group + (blockIdx.y % a.q_chunks) * kHeads;
+  const int nq = min(kHeads, (hk + 1) * a.group - h0);
   const int len = live_length(a.seqlens, b, a.max_len);
   const int start = split * a.chunk, end = min(start + a.chunk, len);
   T* out = (T*)a.out + ((int64_t)b * a.n_heads + h0) * D;
@@ -278,45 +426,65 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
   if (lane == 0)
     for (int i = 0; i < min(n_tiles, kStages); ++i) load(i);
 
-  // q as B operands: lane (g, t) holds head g's elements of K words [W t, W t + W).
+  // q as B operands: lane (g, t) holds column g's elements of K words [W t, W t + W).
   uint32_t qf[NT][2 * W][2];
-  float qsum[NT][2];
+  float qscale[NT][NJ], qsum[NT][NJ];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int h = nt * 8 + g;
-    float sum = 0.f;
+    const int h = NJ == 2 ? nt * 8 + g : (g & 1) ? nq : nt * 4 + g / 2;
+    uint4 raw[W];
+    float sum = 0.f, big = 0.f;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      uint4 raw = make_uint4(0, 0, 0, 0);
+      raw[w] = make_uint4(0, 0, 0, 0);
       if (h < nq)
-        raw = *reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)b * a.q_stride +
-                                              (int64_t)(h0 + h) * D + (t * W + w) * 8);
-      const T* e = reinterpret_cast<const T*>(&raw);
+        raw[w] = *reinterpret_cast<const uint4*>((const T*)a.q + (int64_t)b * a.q_stride +
+                                                 (int64_t)(h0 + h) * D + (t * W + w) * 8);
+      const T* e = reinterpret_cast<const T*>(&raw[w]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += DT<T>::to_f(e[i]);
-      // elements (0,4), (1,5) and (2,6), (3,7): the order pair<E> gives the codes
-      qf[nt][2 * w][0] = __byte_perm(raw.x, raw.z, 0x5410);
-      qf[nt][2 * w][1] = __byte_perm(raw.x, raw.z, 0x7632);
-      qf[nt][2 * w + 1][0] = __byte_perm(raw.y, raw.w, 0x5410);
-      qf[nt][2 * w + 1][1] = __byte_perm(raw.y, raw.w, 0x7632);
+      for (int i = 0; i < 8; ++i) {
+        const float x = DT<T>::to_f(e[i]);
+        sum += x;
+        big = fmaxf(big, fabsf(x));
+      }
     }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    qsum[nt][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-    qsum[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+    }
+    // 2^e brings the largest element into [2^9, 2^10); e stays inside f32's exponents.
+    const int e = min(max((int)((__float_as_uint(big) >> 23) & 0xff) - 127, -100), 100);
+    const float f = __uint_as_float((uint32_t)(127 + 9 - e) << 23);
+    const float back = __uint_as_float((uint32_t)(127 - 9 + e) << 23) * 1048576.f;  // * 2^20
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const T* q = reinterpret_cast<const T*>(&raw[w]);
+      auto at = [&](int i) { return DT<T>::to_f(q[i]) * f; };
+      qf[nt][2 * w][0] = pack2<__half>(at(0) * 16.f, at(4) * 16.f);
+      qf[nt][2 * w][1] = pack2<__half>(at(1), at(5));
+      qf[nt][2 * w + 1][0] = pack2<__half>(at(2) * 16.f, at(6) * 16.f);
+      qf[nt][2 * w + 1][1] = pack2<__half>(at(3), at(7));
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      qsum[nt][j] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * j);
+      qscale[nt][j] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * j);
+    }
   }
 
-  // Per lane, for query heads 2t and 2t + 1 of each tile of eight: running maximum (the same in all
-  // lanes of equal t), this lane's share of the sums, and the output elements of its rows.
-  float m[NT][2], l[NT][2], z[NT][2], o[NT][OT][4];
+  Softmax<D, NT, NJ> st;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = -INFINITY;
-    l[nt][0] = l[nt][1] = z[nt][0] = z[nt][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      st.r[nt][j] = -INFINITY;
+      st.l[nt][j] = st.z[nt][j] = 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.f;
+      for (int j = 0; j < 4; ++j) st.o[nt][i][j] = 0.f;
   }
 
   int done = 0;
@@ -324,141 +492,11 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
     const int stage = done % kStages;
     if (!mbar_wait_warp(&full[warp][stage], (done / kStages) & 1)) break;
     const uint8_t* tile = ring + stage * (kTile * kRec);
-    const int n = min(kTile, end - (first + done * (kWarps * kTile)));
-    float s[2][NT][4];
-    float4 meta[2][2];
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      const uint8_t* r0 = tile + (sub * 16 + g) * kRec;
-      const uint8_t* r1 = r0 + 8 * kRec;
-      uint32_t k0[W], k1[W];
-      if constexpr (W == 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(r0 + 16 * t), y = *reinterpret_cast<const uint4*>(r1 + 16 * t);
-        k0[0] = x.x, k0[1] = x.y, k0[2] = x.z, k0[3] = x.w;
-        k1[0] = y.x, k1[1] = y.y, k1[2] = y.z, k1[3] = y.w;
-      } else if constexpr (W == 2) {
-        const uint2 x = *reinterpret_cast<const uint2*>(r0 + 8 * t), y = *reinterpret_cast<const uint2*>(r1 + 8 * t);
-        k0[0] = x.x, k0[1] = x.y, k1[0] = y.x, k1[1] = y.y;
-      } else {
-        k0[0] = *reinterpret_cast<const uint32_t*>(r0 + 4 * t);
-        k1[0] = *reinterpret_cast<const uint32_t*>(r1 + 4 * t);
-      }
-      meta[sub][0] = *reinterpret_cast<const float4*>(r0 + D);
-      meta[sub][1] = *reinterpret_cast<const float4*>(r1 + D);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[sub][nt][j] = 0.f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const uint32_t lo[4] = {Codes<T>::template pair<0>(k0[w]), Codes<T>::template pair<0>(k1[w]),
-                                Codes<T>::template pair<1>(k0[w]), Codes<T>::template pair<1>(k1[w])};
-        const uint32_t hi[4] = {Codes<T>::template pair<2>(k0[w]), Codes<T>::template pair<2>(k1[w]),
-                                Codes<T>::template pair<3>(k0[w]), Codes<T>::template pair<3>(k1[w])};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma16816<T>(s[sub][nt], lo, qf[nt][2 * w][0], qf[nt][2 * w][1]);
-          mma16816<T>(s[sub][nt], hi, qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
-        }
-      }
-    }
-    // Scores in base 2, and the tile's maximum per query head.
-    float top[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) top[nt][0] = top[nt][1] = -INFINITY;
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float ks = meta[sub][r].x * a.scale_log2;
-        const float km = meta[sub][r].y * a.scale_log2 - kBias * ks;
-        const bool live = sub * 16 + r * 8 + g < n;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float& x = s[sub][nt][2 * r + j];
-            x = live ? fmaf(ks, x, km * qsum[nt][j]) : -INFINITY;
-            top[nt][j] = fmaxf(top[nt][j], x);
-          }
-      }
-    bool grows = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1)
-          top[nt][j] = fmaxf(top[nt][j], __shfl_xor_sync(0xffffffffu, top[nt][j], x));
-        grows |= top[nt][j] > m[nt][j] + 8.f;
-      }
-    // The reference m follows the maximum only when it is left behind by more than 2^8: until then p
-    // stays below 2^8, which f32 sums and the final quotient do not notice.
-    if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float next = fmaxf(m[nt][j], top[nt][j]);
-          const float f = ex2_approx(m[nt][j] - next);
-          m[nt][j] = next;
-          l[nt][j] *= f;
-          z[nt][j] *= f;
-#pragma unroll
-          for (int i = 0; i < OT; ++i) o[nt][i][j] *= f, o[nt][i][2 + j] *= f;
-        }
-    }
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      uint32_t bh[NT][2], bl[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const bool live = sub * 16 + r * 8 + g < n;
-          float hi[2], lo[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float p = live ? ex2_approx(s[sub][nt][2 * r + j] - m[nt][j]) : 0.f;
-            const float pv = live ? p * meta[sub][r].z : 0.f;  // stale scales may be NaN
-            hi[j] = round_to<__nv_bfloat16>(pv);
-            lo[j] = round_to<__nv_bfloat16>(pv - hi[j]);
-            l[nt][j] += p;
-            z[nt][j] += (live ? p * meta[sub][r].w : 0.f) - kBiasV * (hi[j] + lo[j]);
-          }
-          bh[nt][r] = transpose8x8(pack2<__nv_bfloat16>(hi[0], hi[1]));
-          bl[nt][r] = transpose8x8(pack2<__nv_bfloat16>(lo[0], lo[1]));
-        }
-      // V codes of positions 2t, 2t + 1, 2t + 8, 2t + 9: lane (g, t) takes bytes [D/16 g, D/16 (g + 1)).
-      const uint8_t* v = tile + (sub * 16 + 2 * t) * kRec + D / 2 + (D / 16) * g;
-      constexpr int VW = D >= 64 ? D / 64 : 1;
-      uint32_t vw[4][VW];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t* at = v + ((i & 1) + 8 * (i >> 1)) * kRec;
-        if constexpr (D == 128) {
-          const uint2 x = *reinterpret_cast<const uint2*>(at);
-          vw[i][0] = x.x, vw[i][1] = x.y;
-        } else if constexpr (D == 64) {
-          vw[i][0] = *reinterpret_cast<const uint32_t*>(at);
-        } else {
-          vw[i][0] = *reinterpret_cast<const uint16_t*>(at);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < OT; ++i) {
-        const uint32_t sel = (i % 4) * 0x0011u + (4 + i % 4) * 0x1100u;
-        const uint32_t x = __byte_perm(vw[0][i / 4], vw[1][i / 4], sel);
-        const uint32_t y = __byte_perm(vw[2][i / 4], vw[3][i / 4], sel);
-        const uint32_t av[4] = {(x & 0x000f000fu) | 0x43004300u, ((x >> 4) & 0x000f000fu) | 0x43004300u,
-                                (y & 0x000f000fu) | 0x43004300u, ((y >> 4) & 0x000f000fu) | 0x43004300u};
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma16816<__nv_bfloat16>(o[nt][i], av, bh[nt][0], bh[nt][1]);
-          mma16816<__nv_bfloat16>(o[nt][i], av, bl[nt][0], bl[nt][1]);
-        }
-      }
-    }
+    const int n = end - (first + done * (kWarps * kTile));
+    if (n >= kTile)
+      attend_tile<T, D, NT, NJ, true>(tile, kTile, a.scale_log2, qf, qscale, qsum, st);
+    else
+      attend_tile<T, D, NT, NJ, false>(tile, n, a.scale_log2, qf, qscale, qsum, st);
     __syncwarp();
     if (lane == 0 && done + kStages < n_tiles) load(done + kStages);
   }
@@ -470,24 +508,26 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int j = 0; j < NJ; ++j) {
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) {
-        l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], x);
-        z[nt][j] += __shfl_xor_sync(0xffffffffu, z[nt][j], x);
+        st.l[nt][j] += __shfl_xor_sync(0xffffffffu, st.l[nt][j], x);
+        st.z[nt][j] += __shfl_xor_sync(0xffffffffu, st.z[nt][j], x);
       }
-      if (g == 0) sm_m[warp][nt * 8 + 2 * t + j] = m[nt][j], sm_l[warp][nt * 8 + 2 * t + j] = l[nt][j];
+      const int h = (nt * 4 + t) * NJ + j;
+      if (g == 0) sm_m[warp][h] = st.r[nt][j], sm_l[warp][h] = st.l[nt][j];
     }
   __syncthreads();
-  float* sm_o = reinterpret_cast<float*>(smem);  // [kWarps][NT * 8][D]
+  float* sm_o = reinterpret_cast<float*>(smem);  // [kWarps][kHeads][D]
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        *reinterpret_cast<float2*>(sm_o + (warp * NT * 8 + nt * 8 + 2 * t + j) * D + (D / 8) * g + 2 * i) =
-            make_float2(o[nt][i][j] + z[nt][j], o[nt][i][2 + j] + z[nt][j]);
+      for (int j = 0; j < NJ; ++j)
+        *reinterpret_cast<float2*>(sm_o + (warp * kHeads + (nt * 4 + t) * NJ + j) * D + (D / 8) * g + 2 * i) =
+            make_float2(fmaf(st.o[nt][i][j], 16777216.f, st.z[nt][j]),
+                        fmaf(st.o[nt][i][2 + j], 1048576.f, st.z[nt][j]));
   __syncthreads();
   for (int i = tid; i < nq * D; i += kThreads) {
     const int q = i / D;
@@ -500,7 +540,7 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
       if (start + w * kTile >= end) continue;  // this warp had no positions
       const float f = exp2f(sm_m[w][q] - M);
       L += f * sm_l[w][q];
-      O += f * sm_o[(w * NT * 8) * D + i];
+      O += f * sm_o[w * kHeads * D + i];
     }
     if (a.splits == 1) {
       out[i] = DT<T>::from_f(O / L);
@@ -547,11 +587,11 @@ Plan plan(int64_t batch, int64_t n_heads, int64_t n_heads_kv, int64_t max_len) {
   return {(int)(per * 128), (int)((steps + per - 1) / per)};
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int NJ>
 int launch_mma(Args& a, int64_t batch, int64_t n_heads_kv, cudaStream_t stream) {
-  a.q_chunks = ceil_div(a.group, NT * 8);
+  a.q_chunks = ceil_div(a.group, NT * 4 * NJ);
   constexpr int smem = McSmem<D, NT>::kBytes;
-  auto kern = decode_q4_mma_kernel<T, D, NT>;
+  auto kern = decode_q4_mma_kernel<T, D, NT, NJ>;
   if (smem > 48 * 1024)
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   const dim3 grid((unsigned)a.splits, (unsigned)(n_heads_kv * a.q_chunks), (unsigned)batch);
@@ -563,8 +603,9 @@ template <typename T, int D>
 int launch(Args a, int64_t batch, int64_t n_heads_kv, cudaStream_t stream) {
   int s;
   if constexpr (sizeof(T) == 2) {
-    s = a.group > 8 ? launch_mma<T, D, 2>(a, batch, n_heads_kv, stream)
-                    : launch_mma<T, D, 1>(a, batch, n_heads_kv, stream);
+    s = a.group > 8   ? launch_mma<T, D, 2, 2>(a, batch, n_heads_kv, stream)
+        : a.group > 4 ? launch_mma<T, D, 1, 2>(a, batch, n_heads_kv, stream)
+                      : launch_mma<T, D, 1, 1>(a, batch, n_heads_kv, stream);
   } else {
     const dim3 grid((unsigned)a.splits, (unsigned)(n_heads_kv * a.q_chunks), (unsigned)batch);
     s = hx::cuda_status(launch_ex(decode_q4_kernel<T, D>, grid, dim3(kThreads), 0, stream, 1, a),
