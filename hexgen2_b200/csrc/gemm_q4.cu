@@ -76,48 +76,47 @@ __global__ void __launch_bounds__(kThreads) gemm_q4_kernel(const Args p) {
 }
 
 // ------------------------------------------------------------------------------------------
-// Tensor-core kernel (f16/bf16) on mma.m16n8k16 with f32 sums: the 16 rows of A are weight rows, its 8
-// columns rows of a. A code goes in as an exact 16-bit float: bf16 128 + code (OR into the mantissa),
-// f16 code * 2^-24 (its bits are the subnormal); the constant's share, and that of the 8 that codes
-// are offset by, is kOffset * sum of a's group, subtracted with the group's scale in f32.
-//   - A unit is 16 weight rows x 128 k. Nibbles 16 bits apart make one operand register, and the
-//     order of k inside a group is free, so a lane reads whole words of its two rows straight from
-//     global memory (16 bytes at groups of 128), four units ahead.
-//   - a is staged in shared memory in the order of the B operands (one 16-byte load per two
-//     mma), with its group sums.
-//   - A CTA holds 128 weight rows, eight warps of 16. K is split over the S CTAs of a cluster; each
-//     leaves f32 partials in its shared memory and CTA s adds up rows s, s + S, ... of the batch in rank
-//     order, applies the epilogue and stores 128 neighbouring outputs at a time.
+// Tensor-core kernel (f16/bf16) on mma.m16n8k16 with f16 operands and f32 sums: the 16 rows of A are
+// weight rows, its 8 columns rows of a.
+//   - The bits of a code are an f16 as they stand: below 2^11 an f16's value is its bits times 2^-24
+//     (subnormals and the first binade). A masked word is an operand register: w & 0x000f000f
+//     holds codes * 2^-24, w & 0x00f000f0 codes * 2^-20; nothing is converted or rounded, and the
+//     8 that codes are offset by comes off with the group's sum of a, in f32.
+//   - a goes in as f16 times a power of two of its own per (row, 128 k): max |a| in [2^9, 2^10), times 16
+//     where the codes are not, so bf16 and f16 values down to 2^-24 of the unit's largest are exact
+//     (smaller ones to 2^-35 of it). The factor comes off with the group's scale.
+//   - A unit is 16 weight rows x 128 k. Nibbles 16 bits apart make one operand register, and the order of
+//     k inside a group is free, so a lane reads whole words of its two rows straight from global
+//     memory (16 bytes at groups of 128), four units ahead.
+//   - a is staged in the order of the B operands (one 16-byte load feeds two mma) with its group
+//     sums and factors: by every CTA for its own slice up to eight rows; above, once by
+//     stage_kernel, and warp 0 keeps a ring of its blocks filled.
+//   - A CTA has `warps` warps of 16 weight rows. K is split over the S CTAs of a cluster; each leaves
+//     f32 partials in its shared memory and CTA s adds up rows s, s + S, ... of the batch in rank
+//     order, applies the epilogue and stores neighbouring outputs together.
 // ------------------------------------------------------------------------------------------
-constexpr int kMmaThreads = 256;
-constexpr int kRows = 128;   // weight rows per CTA
+constexpr int kMaxWarps = 8;
 constexpr int kUnitK = 128;
-constexpr int kPitch = kRows + 4;
+constexpr int kStages = 4;   // ring of staged blocks of a
+constexpr int kChunk = 32;   // units staged at a time up to eight rows
 
-template <typename T> struct Codes;
-template <> struct Codes<__nv_bfloat16> {
-  static constexpr float kOffset = 136.f, kScale = 1.f;
-  static HX_DEVICE uint32_t pair(uint32_t w, int e) { return ((w >> (4 * e)) & 0x000f000fu) | 0x43004300u; }
-  static HX_DEVICE void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-template <> struct Codes<__half> {
-  static constexpr float kOffset = 8.f / 16777216.f, kScale = 16777216.f;
-  static HX_DEVICE uint32_t pair(uint32_t w, int e) { return (w >> (4 * e)) & 0x000f000fu; }
-  static HX_DEVICE void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
+// One unit of a: operands [NT][4 words][8 rows][4 lanes] x 16 bytes, then [groups][NT * 8] (offset, factor).
+template <int G, int NT>
+struct Block {
+  static constexpr int kAhead = NT == 8 || G == 32 ? 2 : 4;  // units in flight per warp
+  static constexpr int kPerStage = 8 / NT < kAhead ? 8 / NT : kAhead;
+  static constexpr int kGroups = kUnitK / G;
+  static constexpr int kOperands = NT * 2048;
+  static constexpr int kBytes = kOperands + kGroups * NT * 8 * 8;
 };
 
+HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 HX_DEVICE uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -139,6 +138,57 @@ HX_DEVICE uint4 ld_stream(const void* p) {
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
+HX_DEVICE void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Elements [8 c, 8 c + 8) of a unit of batch row m (`raw`, zeros where a has none) into its block.
+// Called by whole warps, the 16 lanes of a unit side by side; `live` lanes store.
+template <typename T, int G, int NT>
+HX_DEVICE void stage(uint8_t* block, int m, int c, uint4 raw, bool live) {
+  const T* e = reinterpret_cast<const T*>(&raw);
+  float x[8], sum = 0.f, big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x[i] = DT<T>::to_f(e[i]);
+    sum += x[i];
+    big = fmaxf(big, fabsf(x[i]));
+  }
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) {
+    if (o < G / 8) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  }
+  if (!live) return;
+  const int ex = max((int)((__float_as_uint(big) >> 23) & 0xff) - 127, -100);
+  const float f = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
+  const int at = 8 * c, j = at / G, rest = at % G, t = rest / (G / 4), w = j * (G / 32) + rest % (G / 4) / 8;
+  *reinterpret_cast<uint4*>(block + (((m >> 3) * 4 + w) * 32 + (m & 7) * 4 + t) * 16) =
+      make_uint4(pack2<__half>(x[0] * f * 16.f, x[4] * f * 16.f), pack2<__half>(x[1] * f, x[5] * f),
+                 pack2<__half>(x[2] * f * 16.f, x[6] * f * 16.f), pack2<__half>(x[3] * f, x[7] * f));
+  if (rest == 0)  // (offset, factor) of acc * factor + offset, both times 2^-20
+    *reinterpret_cast<float2*>(block + Block<G, NT>::kOperands + (j * NT * 8 + m) * 8) =
+        make_float2(sum * (-8.f / 1048576.f), __uint_as_float((uint32_t)(127 - 9 + ex) << 23));
+}
+
+template <typename T, int G, int NT>
+__global__ void __launch_bounds__(256) stage_kernel(const Args p, uint8_t* __restrict__ blocks) {
+  pdl_wait();
+  pdl_trigger();
+  const int u = blockIdx.x, c = threadIdx.x & 15;
+  const int64_t k = (int64_t)u * kUnitK + c * 8;
+#pragma unroll
+  for (int m0 = 0; m0 < NT * 8; m0 += 16) {
+    const int m = m0 + (threadIdx.x >> 4);
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (m < p.M && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)m * p.lda + k);
+    stage<T, G, NT>(blocks + (int64_t)u * Block<G, NT>::kBytes, m, c, raw, true);
+  }
+}
 
 // One unit of a lane: the words of rows g and g + 8 and their groups' scales.
 template <typename T, int G>
@@ -147,153 +197,176 @@ struct Unit {
   T s[2][kUnitK / G];
 };
 
-// Byte offset, in a's staged chunk of NT tiles of 8 rows, of elements [8 c, 8 c + 8) of batch row m.
-template <int G, int NT>
-HX_DEVICE int staged(int m, int c) {
-  const int u = c >> 4, in = (c & 15) * 8;
-  const int j = in / G, rest = in % G, t = rest / (G / 4), w = j * (G / 32) + rest % (G / 4) / 8;
-  return (((u * NT + (m >> 3)) * 4 + w) * 32 + (m & 7) * 4 + t) * 16;
+template <typename T, int G, int NT>
+HX_DEVICE void multiply(const Unit<T, G>& x, const uint8_t* block, float (&tot)[NT][4]) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+  for (int j = 0; j < kUnitK / G; ++j) {
+    float acc[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) acc[nt][y] = 0.f;
+#pragma unroll
+    for (int w = j * (G / 32); w < (j + 1) * (G / 32); ++w) {
+      const uint32_t x0 = x.w[0][w], y0 = x.w[1][w], x1 = x0 >> 8, y1 = y0 >> 8;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint4 v = *reinterpret_cast<const uint4*>(block + (nt * 4 + w) * 512 + lane * 16);
+        mma_f16(acc[nt], x0 & 0x000f000fu, y0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x00f000f0u, v.x, v.y);
+        mma_f16(acc[nt], x1 & 0x000f000fu, y1 & 0x000f000fu, x1 & 0x00f000f0u, y1 & 0x00f000f0u, v.z, v.w);
+      }
+    }
+    const float s0 = DT<T>::to_f(x.s[0][j]) * 1048576.f, s1 = DT<T>::to_f(x.s[1][j]) * 1048576.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float4 f = *reinterpret_cast<const float4*>(block + Block<G, NT>::kOperands +
+                                                        (j * NT * 8 + nt * 8 + 2 * t) * 8);
+      tot[nt][0] = fmaf(s0, fmaf(acc[nt][0], f.y, f.x), tot[nt][0]);
+      tot[nt][1] = fmaf(s0, fmaf(acc[nt][1], f.w, f.z), tot[nt][1]);
+      tot[nt][2] = fmaf(s1, fmaf(acc[nt][2], f.y, f.x), tot[nt][2]);
+      tot[nt][3] = fmaf(s1, fmaf(acc[nt][3], f.w, f.z), tot[nt][3]);
+    }
+  }
 }
 
 template <typename T, int G, int NT, int EPI>
-__global__ void __launch_bounds__(kMmaThreads, NT == 8 ? 1 : 2) gemm_q4_mma_kernel(const Args p, int S, int chunk_units) {
-  constexpr int kAhead = 4;       // units in flight per warp
-  constexpr int GU = kUnitK / G;  // groups per unit
+__global__ void __launch_bounds__(kMaxWarps * 32, 2) gemm_q4_mma_kernel(
+    const Args p, const uint8_t* __restrict__ blocks, int S, int warps) {
+  using B = Block<G, NT>;
+  constexpr bool kRing = NT > 1;
+  constexpr int kPerStage = B::kPerStage, kAhead = B::kAhead;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint8_t* sm_a = smem;                                                     // chunk_units * NT * 2 KB
-  float* sm_sum = reinterpret_cast<float*>(smem + chunk_units * NT * 2048);  // [groups][NT * 8]
+  __shared__ uint64_t full[kStages], empty[kStages];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (kRing) {
+    if (tid == 0) {
+      for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], warps);
+      fence_mbar_init();
+    }
+    __syncthreads();
+  }
   pdl_wait();
   pdl_trigger();
   const int rank = S > 1 ? (int)cluster_rank() : 0;
-  const int n0 = (blockIdx.x / S) * kRows;
+  const int rows = warps * 16, n0 = (int)(blockIdx.x / S) * rows;
   const int units = (p.K + kUnitK - 1) / kUnitK;
   const int begin = (int)((int64_t)units * rank / S), end = (int)((int64_t)units * (rank + 1) / S);
-  const int groups = p.K / G;
-  const int row = n0 + warp * 16 + g;
-  const bool in[2] = {row < p.N, row + 8 < p.N};
-  const uint8_t* wp = p.w + (int64_t)row * (p.K / 2);
-  const T* sp = (const T*)p.scales + (int64_t)row * groups;
-  using U = Unit<T, G>;
-  auto fetch = [&](U& x, int u) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const uint8_t* base = wp + (int64_t)r * 8 * (p.K / 2) + (int64_t)u * (kUnitK / 2);
-#pragma unroll
-      for (int j = 0; j < GU; ++j) {
-        const int grp = u * GU + j;
-        const bool some = in[r] && u < end && grp < groups;
-        if constexpr (G == 128) {
-          const uint4 v = some ? ld_stream(base + 16 * t) : make_uint4(0, 0, 0, 0);
-          x.w[r][0] = v.x, x.w[r][1] = v.y, x.w[r][2] = v.z, x.w[r][3] = v.w;
-        } else if constexpr (G == 64) {
-          const uint2 v = some ? __ldg(reinterpret_cast<const uint2*>(base + 32 * j + 8 * t)) : make_uint2(0, 0);
-          x.w[r][2 * j] = v.x, x.w[r][2 * j + 1] = v.y;
-        } else {
-          x.w[r][j] = some ? __ldg(reinterpret_cast<const uint32_t*>(base + 16 * j + 4 * t)) : 0u;
-        }
-        x.s[r][j] = some ? __ldg(sp + (int64_t)r * 8 * groups + grp) : DT<T>::from_f(0.f);
-      }
-    }
-  };
-  U buf[kAhead];
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) fetch(buf[i], begin + i);
-
   float tot[NT][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int j = 0; j < 4; ++j) tot[nt][j] = 0.f;
 
-  for (int c0 = begin; c0 < end; c0 += chunk_units) {
-    const int nu = min(chunk_units, end - c0);
-    // Stage a's chunk: 16 bytes a thread, neighbouring threads along k, group sums over G / 8 lanes.
-    if (c0 != begin) __syncthreads();
-    const int per_row = nu * 16, items = p.M * per_row;
-    for (int i0 = 0; i0 < items; i0 += kMmaThreads) {
-      const int i = i0 + tid;
-      const int m = min(i / per_row, p.M - 1), c = i - i / per_row * per_row;
-      const int64_t k = (int64_t)c0 * kUnitK + c * 8;
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (i < items && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)m * p.lda + k);
-      const T* e = reinterpret_cast<const T*>(&raw);
-      float sum = 0.f;
+  // Warp 0's lane 0: the next stage of a's blocks, once every warp has left the stage it replaces.
+  bool ok = true;
+  int asked = 0;
+  auto ask = [&]() {
+    const int u = begin + asked * kPerStage, st = asked % kStages;
+    if (u >= end || !ok) return;
+    if (asked >= kStages && !(ok = mbar_wait(&empty[st], (asked / kStages - 1) & 1))) return;
+    const uint32_t bytes = (uint32_t)min(kPerStage, end - u) * B::kBytes;
+    mbar_arrive_expect_tx(&full[st], bytes);
+    bulk_load(smem + st * (kPerStage * B::kBytes), blocks + (int64_t)u * B::kBytes, bytes, &full[st]);
+    ++asked;
+  };
+  if (kRing && tid == 0)
+    for (int i = 0; i < kStages - 1; ++i) ask();
+  {
+    // Rows past N read row N - 1 and are not stored; groups past K (units are whole) read the last one
+    // and meet zeros of a.
+    const int groups = p.K / G, row0 = min(n0 + warp * 16 + g, p.N - 1), row1 = min(n0 + warp * 16 + g + 8, p.N - 1);
+    const uint8_t* wp[2] = {p.w + (int64_t)row0 * (p.K / 2) + t * (G / 8), p.w + (int64_t)row1 * (p.K / 2) + t * (G / 8)};
+    const T* sp[2] = {(const T*)p.scales + (int64_t)row0 * groups, (const T*)p.scales + (int64_t)row1 * groups};
+    using U = Unit<T, G>;
+    auto fetch = [&](U& x, int u) {
+      u = min(u, end - 1);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) sum += DT<T>::to_f(e[x]);
+      for (int j = 0; j < B::kGroups; ++j) {
+        const int grp = G == 128 ? u : min(u * B::kGroups + j, groups - 1);
 #pragma unroll
-      for (int o = 1; o < G / 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (i < items) {
-        *reinterpret_cast<uint4*>(sm_a + staged<G, NT>(m, c)) =
-            make_uint4(__byte_perm(raw.x, raw.z, 0x5410), __byte_perm(raw.x, raw.z, 0x7632),
-                       __byte_perm(raw.y, raw.w, 0x5410), __byte_perm(raw.y, raw.w, 0x7632));
-        if (c % (G / 8) == 0) sm_sum[(c / (G / 8)) * (NT * 8) + m] = sum;
-      }
-    }
-    __syncthreads();
-    for (int u = 0; u < nu; u += kAhead) {
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        if (u + i >= nu) break;
-        const U x = buf[i];
-        const uint8_t* b = sm_a + (u + i) * (NT * 2048) + lane * 16;
-#pragma unroll
-        for (int j = 0; j < GU; ++j) {
-          float acc[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) acc[nt][y] = 0.f;
-#pragma unroll
-          for (int w = j * (G / 32); w < (j + 1) * (G / 32); ++w) {
-            const uint32_t lo[4] = {Codes<T>::pair(x.w[0][w], 0), Codes<T>::pair(x.w[1][w], 0),
-                                    Codes<T>::pair(x.w[0][w], 1), Codes<T>::pair(x.w[1][w], 1)};
-            const uint32_t hi[4] = {Codes<T>::pair(x.w[0][w], 2), Codes<T>::pair(x.w[1][w], 2),
-                                    Codes<T>::pair(x.w[0][w], 3), Codes<T>::pair(x.w[1][w], 3)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint4 v = *reinterpret_cast<const uint4*>(b + (nt * 4 + w) * 512);
-              Codes<T>::mma(acc[nt], lo, v.x, v.y);
-              Codes<T>::mma(acc[nt], hi, v.z, v.w);
-            }
+        for (int r = 0; r < 2; ++r) {
+          const uint8_t* at = wp[r] + grp * (G / 2);
+          if constexpr (G == 128) {
+            const uint4 v = ld_stream(at);
+            x.w[r][0] = v.x, x.w[r][1] = v.y, x.w[r][2] = v.z, x.w[r][3] = v.w;
+          } else if constexpr (G == 64) {
+            const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+            x.w[r][2 * j] = v.x, x.w[r][2 * j + 1] = v.y;
+          } else {
+            x.w[r][j] = __ldg(reinterpret_cast<const uint32_t*>(at));
           }
-          const float s0 = DT<T>::to_f(x.s[0][j]) * Codes<T>::kScale, s1 = DT<T>::to_f(x.s[1][j]) * Codes<T>::kScale;
-          const float* sums = sm_sum + ((u + i) * GU + j) * (NT * 8) + 2 * t;
+          x.s[r][j] = __ldg(sp[r] + grp);
+        }
+      }
+    };
+    U buf[kAhead];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float2 sum = *reinterpret_cast<const float2*>(sums + nt * 8);
-            tot[nt][0] = fmaf(s0, fmaf(-Codes<T>::kOffset, sum.x, acc[nt][0]), tot[nt][0]);
-            tot[nt][1] = fmaf(s0, fmaf(-Codes<T>::kOffset, sum.y, acc[nt][1]), tot[nt][1]);
-            tot[nt][2] = fmaf(s1, fmaf(-Codes<T>::kOffset, sum.x, acc[nt][2]), tot[nt][2]);
-            tot[nt][3] = fmaf(s1, fmaf(-Codes<T>::kOffset, sum.y, acc[nt][3]), tot[nt][3]);
+    for (int i = 0; i < kAhead; ++i) fetch(buf[i], begin + i);
+    int st = 0, phase = 0;
+    for (int c0 = begin; c0 < end; c0 += kRing ? end - begin : kChunk) {
+      const int c1 = kRing ? end : min(end, c0 + kChunk);
+      if (!kRing) {  // stage a's slice: 16 bytes a thread, neighbouring threads along k
+        if (c0 != begin) __syncthreads();
+        const int per_row = (c1 - c0) * 16, items = p.M * per_row;
+        for (int i0 = 0; i0 < items; i0 += warps * 32) {
+          const int i = i0 + tid, m = min(i / per_row, p.M - 1), c = i - i / per_row * per_row;
+          const int64_t k = (int64_t)c0 * kUnitK + c * 8;
+          uint4 raw = make_uint4(0, 0, 0, 0);
+          if (i < items && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)m * p.lda + k);
+          stage<T, G, NT>(smem + (c >> 4) * B::kBytes, m, c & 15, raw, i < items);
+        }
+        __syncthreads();
+      }
+      for (int u = c0; u < c1 && ok; u += kAhead) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (u + i >= c1) break;
+          if (kRing && i % kPerStage == 0) {
+            if (tid == 0) ask();
+            ok = mbar_wait_warp(&full[st], phase) && __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+          }
+          const uint8_t* block = kRing ? smem + (st * kPerStage + i % kPerStage) * B::kBytes
+                                       : smem + (u + i - c0) * B::kBytes;
+          multiply<T, G, NT>(buf[i], block, tot);
+          fetch(buf[i], u + i + kAhead);
+          if (kRing && (i % kPerStage == kPerStage - 1 || u + i + 1 == end)) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+            if (++st == kStages) st = 0, phase ^= 1;
           }
         }
-        fetch(buf[i], c0 + u + i + kAhead);
       }
     }
   }
 
+  if (kRing && tid == 0 && !ok)  // a wait gave up: let the copies in flight land
+    for (int i = max(0, asked - kStages); i < asked; ++i) mbar_wait_drain(&full[i % kStages], (i / kStages) & 1);
+
   // Partials [batch row][weight row] in shared memory, added up over the cluster.
   __syncthreads();
   float* part = reinterpret_cast<float*>(smem);
+  const int pitch = rows + 4;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      part[(nt * 8 + 2 * t + (j & 1)) * kPitch + warp * 16 + g + 8 * (j >> 1)] = tot[nt][j];
+      part[(nt * 8 + 2 * t + (j & 1)) * pitch + warp * 16 + g + 8 * (j >> 1)] = tot[nt][j];
   if (S > 1) cluster_sync(); else __syncthreads();
-  constexpr int kCols = EPI == HX_EPI_SWIGLU ? kRows / 2 : kRows;
+  const int width = EPI == HX_EPI_SWIGLU ? rows / 2 : rows;  // outputs of one batch row in this CTA
   const int cols = EPI == HX_EPI_SWIGLU ? p.N / 2 : p.N, col0 = EPI == HX_EPI_SWIGLU ? n0 / 2 : n0;
   auto total = [&](int m, int r) {
-    const float* at = part + m * kPitch + r;
+    const float* at = part + m * pitch + r;
     if (S == 1) return *at;
     float v = 0.f;
     for (int s = 0; s < S; ++s) v += ld_cluster_f32(smem_u32(at), s);
     return v;
   };
-  const int c = tid % kCols;
-  for (int m = rank + S * (tid / kCols); m < p.M; m += S * (kMmaThreads / kCols)) {
-    if (col0 + c >= cols) break;
+  const int mine = (p.M - rank + S - 1) / S * width;  // rows rank, rank + S, ...
+  for (int i = tid; i < mine; i += blockDim.x) {
+    const int m = rank + S * (i / width), c = i % width;
+    if (col0 + c >= cols) continue;
     float v;
     if constexpr (EPI == HX_EPI_SWIGLU) {
       const int r = (c / 16) * 32 + c % 16;
@@ -307,40 +380,71 @@ __global__ void __launch_bounds__(kMmaThreads, NT == 8 ? 1 : 2) gemm_q4_mma_kern
   if (S > 1) cluster_sync();  // no CTA leaves while others read its partials
 }
 
+int tiles_of(int64_t m) { return m <= 8 ? 1 : m <= 16 ? 2 : m <= 32 ? 4 : 8; }
+
+// Warps per CTA and CTAs per cluster: the pair whose fullest SM has the least to do, a CTA counting
+// its 16-row tiles times its units of K plus what it takes to start and to store (about 16 of those).
+struct Plan {
+  int warps, S;
+};
+Plan plan(int64_t n, int64_t k, bool pairs) {
+  const int tiles = ceil_div(n, 16), units = ceil_div(k, kUnitK);
+  Plan best{kMaxWarps, 1};
+  int64_t least = INT64_MAX;
+  for (int warps = kMaxWarps; warps >= 4; warps -= pairs ? 2 : 1)
+    for (int S = 1; S <= 8 && (S == 1 || 2 * S <= units); ++S) {
+      const int64_t ctas = (int64_t)ceil_div(tiles, warps) * S;
+      const int64_t cost = ceil_div(ctas, 148) * ((int64_t)warps * ceil_div(units, S) + 16);
+      if (cost < least) least = cost, best = {warps, S};
+    }
+  return best;
+}
+
 template <typename T, int G, int NT, int EPI>
-int launch_mma(const Args& p, cudaStream_t stream) {
-  const int blocks = ceil_div(p.N, kRows), units = ceil_div(p.K, kUnitK);
-  const int S = std::max(1, std::min({8, 2 * 148 / blocks, units / 2}));
-  const int chunk = std::min(32 / NT, ceil_div(units, S));
-  const size_t stage = (size_t)chunk * NT * 2048 + (size_t)chunk * (kUnitK / G) * NT * 8 * sizeof(float);
-  const size_t smem = std::max(stage, (size_t)NT * 8 * kPitch * sizeof(float));
+int launch_mma(const Args& p, uint8_t* blocks, cudaStream_t stream) {
+  using B = Block<G, NT>;
+  const Plan pl = plan(p.N, p.K, EPI == HX_EPI_SWIGLU);
+  const int units = ceil_div(p.K, kUnitK);
+  if (NT > 1) {
+    const int s = hx::cuda_status(launch_ex(stage_kernel<T, G, NT>, dim3((unsigned)units), dim3(256), 0, stream, 1, p, blocks),
+                                  "gemm_q4 stage_kernel launch");
+    if (s) return s;
+  }
+  const size_t staged = NT > 1 ? (size_t)kStages * B::kPerStage * B::kBytes
+                               : (size_t)std::min(kChunk, ceil_div(units, pl.S)) * B::kBytes;
+  const size_t smem = std::max(staged, (size_t)NT * 8 * (pl.warps * 16 + 4) * sizeof(float));
   auto kern = gemm_q4_mma_kernel<T, G, NT, EPI>;
-  if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 72 * 1024);
-  return hx::cuda_status(launch_ex(kern, dim3((unsigned)(blocks * S)), dim3(kMmaThreads), smem, stream, S, p, S, chunk),
-                         "gemm_q4_mma_kernel launch");
+  if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+  return hx::cuda_status(
+      launch_ex(kern, dim3((unsigned)(ceil_div(p.N, pl.warps * 16) * pl.S)),
+                dim3((unsigned)(pl.warps * 32)), smem, stream, pl.S, p,
+                (const uint8_t*)blocks, pl.S, pl.warps),
+      "gemm_q4_mma_kernel launch");
 }
 
 template <typename T, int G, int NT>
-int launch_epilogue(const Args& p, int epilogue, cudaStream_t stream) {
-  return epilogue == HX_EPI_SWIGLU     ? launch_mma<T, G, NT, HX_EPI_SWIGLU>(p, stream)
-         : epilogue == HX_EPI_RESIDUAL ? launch_mma<T, G, NT, HX_EPI_RESIDUAL>(p, stream)
-                                       : launch_mma<T, G, NT, HX_EPI_NONE>(p, stream);
+int launch_epilogue(const Args& p, int epilogue, uint8_t* blocks, cudaStream_t stream) {
+  return epilogue == HX_EPI_SWIGLU     ? launch_mma<T, G, NT, HX_EPI_SWIGLU>(p, blocks, stream)
+         : epilogue == HX_EPI_RESIDUAL ? launch_mma<T, G, NT, HX_EPI_RESIDUAL>(p, blocks, stream)
+                                       : launch_mma<T, G, NT, HX_EPI_NONE>(p, blocks, stream);
 }
 
 template <typename T, int G>
-int launch_rows(const Args& p, int epilogue, cudaStream_t stream) {
-  return p.M <= 8    ? launch_epilogue<T, G, 1>(p, epilogue, stream)
-         : p.M <= 16 ? launch_epilogue<T, G, 2>(p, epilogue, stream)
-         : p.M <= 32 ? launch_epilogue<T, G, 4>(p, epilogue, stream)
-                     : launch_epilogue<T, G, 8>(p, epilogue, stream);
+int launch_rows(const Args& p, int epilogue, uint8_t* blocks, cudaStream_t stream) {
+  switch (tiles_of(p.M)) {
+    case 1: return launch_epilogue<T, G, 1>(p, epilogue, blocks, stream);
+    case 2: return launch_epilogue<T, G, 2>(p, epilogue, blocks, stream);
+    case 4: return launch_epilogue<T, G, 4>(p, epilogue, blocks, stream);
+    default: return launch_epilogue<T, G, 8>(p, epilogue, blocks, stream);
+  }
 }
 
 template <typename T>
-int launch(const Args& p, int epilogue, cudaStream_t stream) {
+int launch(const Args& p, int epilogue, uint8_t* blocks, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    return p.group == 128  ? launch_rows<T, 128>(p, epilogue, stream)
-           : p.group == 64 ? launch_rows<T, 64>(p, epilogue, stream)
-                           : launch_rows<T, 32>(p, epilogue, stream);
+    return p.group == 128  ? launch_rows<T, 128>(p, epilogue, blocks, stream)
+           : p.group == 64 ? launch_rows<T, 64>(p, epilogue, blocks, stream)
+                           : launch_rows<T, 32>(p, epilogue, blocks, stream);
   } else {
     const int64_t cols = epilogue == HX_EPI_SWIGLU ? p.N / 2 : p.N;
     const dim3 grid((unsigned)ceil_div(cols, kThreads / 32), (unsigned)ceil_div(p.M, MB));
@@ -354,10 +458,16 @@ int launch(const Args& p, int epilogue, cudaStream_t stream) {
 
 }  // namespace
 
+extern "C" size_t hx_gemm_q4_workspace(int64_t m, int64_t k, int64_t group, int dtype) {
+  if (m <= 8 || m > 64 || k <= 0 || group < 32 || group > kUnitK || dtype == HX_F32) return 0;
+  const size_t nt = (size_t)tiles_of(m);
+  return (size_t)ceil_div(k, kUnitK) * nt * (2048 + (size_t)(kUnitK / group) * 64);
+}
+
 extern "C" int hx_gemm_q4(const void* a, const void* w, const void* scales, void* c, int64_t m,
                           int64_t n, int64_t k, int64_t group, int64_t lda, int64_t ldc,
-                          int epilogue, const void* residual, int64_t ld_residual, int dtype,
-                          void* stream) {
+                          int epilogue, const void* residual, int64_t ld_residual, void* workspace,
+                          size_t workspace_bytes, int dtype, void* stream) {
   HX_REQUIRE(a && w && scales && c, "hx_gemm_q4: null pointer");
   HX_REQUIRE(group == 32 || group == 64 || group == 128,
              "hx_gemm_q4: group %lld unsupported (32, 64 or 128)", (long long)group);
@@ -375,8 +485,11 @@ extern "C" int hx_gemm_q4(const void* a, const void* w, const void* scales, void
   HX_REQUIRE(ldc >= cols && (epilogue != HX_EPI_RESIDUAL || ld_residual >= cols),
              "hx_gemm_q4: bad output or residual stride");
   if (m == 0) return HX_OK;
+  const size_t need = hx_gemm_q4_workspace(m, k, group, dtype);
+  HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
+             "hx_gemm_q4: workspace too small (%zu < %zu) or misaligned", workspace_bytes, need);
   const Args p{a, (const uint8_t*)w, scales, residual, c, lda, ld_residual, ldc,
                (int)m, (int)n, (int)k, (int)group};
-  HX_DISPATCH_DTYPE(dtype, T, return launch<T>(p, epilogue, (cudaStream_t)stream));
+  HX_DISPATCH_DTYPE(dtype, T, return launch<T>(p, epilogue, (uint8_t*)workspace, (cudaStream_t)stream));
   return HX_OK;
 }

@@ -118,15 +118,17 @@ P = 1 << 20  # an aligned address that is never followed: every call below fails
     ("hx_decode_attention_q4", [P, 64, P, 384, 384, P, 1, 2, 1, 40, 8, 1.0, P, None, 0, 0, None]),
     ("hx_decode_attention_q4", [P, 64, P, 384, 384, P, 1, 2, 1, 32, 9, 1.0, P, None, 0, 0, None]),  # beyond
     ("hx_decode_attention_q4", [P, 64, P, 1 << 24, 1 << 24, P, 1, 2, 1, 32, 100000, 1.0, P, P, 16, 0, None]),
-    ("hx_gemm_q4", [P, P, P, P, 65, 32, 64, 32, 64, 32, 0, None, 0, 0, None]),  # rows
-    ("hx_gemm_q4", [P, P, P, P, 1, 32, 96, 64, 96, 32, 0, None, 0, 0, None]),  # k % group
-    ("hx_gemm_q4", [P, P, P, P, 1, 32, 64, 16, 64, 32, 0, None, 0, 0, None]),  # group
-    ("hx_gemm_q4", [P, P, P, P, 1, 48, 64, 32, 64, 48, 2, None, 0, 0, None]),  # SwiGLU n
-    ("hx_gemm_q4", [P, P, P, P, 1, 32, 64, 32, 64, 32, 1, None, 0, 0, None]),  # no residual
-    ("hx_gemm_q4", [P, P, P, P, 1, 32, 64, 32, 64, 32, 3, P, 32, 0, None]),  # epilogue
-    ("hx_gemm_q4", [P, P, P, P, 2, 32, 64, 32, 66, 32, 0, None, 0, 1, None]),  # lda
-    ("hx_gemm_q4", [P, P, P, P, 2, 32, 64, 32, 64, 31, 0, None, 0, 1, None]),  # ldc
-    ("hx_gemm_q4", [P + 4, P, P, P, 1, 32, 64, 32, 64, 32, 0, None, 0, 0, None]),
+    ("hx_gemm_q4", [P, P, P, P, 65, 32, 64, 32, 64, 32, 0, None, 0, P, 1 << 30, 0, None]),  # rows
+    ("hx_gemm_q4", [P, P, P, P, 1, 32, 96, 64, 96, 32, 0, None, 0, P, 1 << 30, 0, None]),  # k % group
+    ("hx_gemm_q4", [P, P, P, P, 1, 32, 64, 16, 64, 32, 0, None, 0, P, 1 << 30, 0, None]),  # group
+    ("hx_gemm_q4", [P, P, P, P, 1, 48, 64, 32, 64, 48, 2, None, 0, P, 1 << 30, 0, None]),  # SwiGLU n
+    ("hx_gemm_q4", [P, P, P, P, 1, 32, 64, 32, 64, 32, 1, None, 0, P, 1 << 30, 0, None]),  # no residual
+    ("hx_gemm_q4", [P, P, P, P, 1, 32, 64, 32, 64, 32, 3, P, 32, P, 1 << 30, 0, None]),  # epilogue
+    ("hx_gemm_q4", [P, P, P, P, 2, 32, 64, 32, 66, 32, 0, None, 0, P, 1 << 30, 1, None]),  # lda
+    ("hx_gemm_q4", [P, P, P, P, 2, 32, 64, 32, 64, 31, 0, None, 0, P, 1 << 30, 1, None]),  # ldc
+    ("hx_gemm_q4", [P + 4, P, P, P, 1, 32, 64, 32, 64, 32, 0, None, 0, P, 1 << 30, 0, None]),
+    ("hx_gemm_q4", [P, P, P, P, 9, 32, 64, 32, 64, 32, 0, None, 0, P, 16, 1, None]),  # workspace
+    ("hx_gemm_q4", [P, P, P, P, 9, 32, 64, 32, 64, 32, 0, None, 0, P + 8, 1 << 30, 1, None]),
     ("hx_token_logprobs", [P, 2, 8, 7, P, 0, P, None, None, None, 0, None]),  # ld
     ("hx_token_logprobs", [P, 2, 8, 8, P, 9, P, None, P, P, 0, None]),  # top_k > cols
     ("hx_token_logprobs", [P, 2, 80, 80, P, 33, P, None, P, P, 0, None]),  # top_k > 32
@@ -141,8 +143,8 @@ def test_c_entry_points_refuse(name, args):
 
 def test_unsupported_dtype_and_empty_calls():
     lib = _lib.lib()
-    assert lib.hx_gemm_q4(P, P, P, P, 1, 32, 64, 32, 64, 32, 0, None, 0, 7, None) == _lib.HX_ERR_UNSUPPORTED
-    assert lib.hx_gemm_q4(P, P, P, P, 0, 32, 64, 32, 64, 32, 0, None, 0, 0, None) == _lib.HX_OK
+    assert lib.hx_gemm_q4(P, P, P, P, 1, 32, 64, 32, 64, 32, 0, None, 0, P, 1 << 30, 7, None) == _lib.HX_ERR_UNSUPPORTED
+    assert lib.hx_gemm_q4(P, P, P, P, 0, 32, 64, 32, 64, 32, 0, None, 0, P, 1 << 30, 0, None) == _lib.HX_OK
     assert lib.hx_token_logprobs(P, 0, 8, 8, P, 0, P, None, None, None, 0, None) == _lib.HX_OK
     assert lib.hx_quantize_cache_q4(P, 64, 64, 8, None, P, 0, 1, 32, P, 384, 384, 0, 8, 0, None) == _lib.HX_OK
 
