@@ -87,7 +87,6 @@ __global__ void __launch_bounds__(kThreads) gemm_q4_kernel(const Args p) {
 //     (smaller ones to 2^-35 of it). The factor comes off with the group's scale.
 //   - A unit is 16 weight rows x 128 k. Nibbles 16 bits apart make one operand register, and the order of
 //     k inside a group is free, so a lane reads whole words of its two rows straight from global
-//     memory (16 bytes at groups of 128), four units ahead.
 //   - a is staged in the order of the B operands (one 16-byte load feeds two mma) with its group
 //     sums and factors: by every CTA for its own slice up to eight rows; above, once by
 //     stage_kernel, and warp 0 keeps a ring of its blocks filled.
@@ -97,17 +96,20 @@ __global__ void __launch_bounds__(kThreads) gemm_q4_kernel(const Args p) {
 // ------------------------------------------------------------------------------------------
 constexpr int kMaxWarps = 8;
 constexpr int kUnitK = 128;
-constexpr int kStages = 4;   // ring of staged blocks of a
-constexpr int kChunk = 32;   // units staged at a time up to eight rows
+constexpr int kPair = 2;     // units per stage of a warp's ring of weights
+constexpr int kStageBytes = 16 * 128;
+constexpr int kChunk = 16;   // units of a staged at a time up to eight rows
 
 // One unit of a: operands [NT][4 words][8 rows][4 lanes] x 16 bytes, then [groups][NT * 8] (offset, factor).
 template <int G, int NT>
 struct Block {
-  static constexpr int kAhead = NT == 8 || G == 32 ? 2 : 4;  // units in flight per warp
-  static constexpr int kPerStage = 8 / NT < kAhead ? 8 / NT : kAhead;
   static constexpr int kGroups = kUnitK / G;
   static constexpr int kOperands = NT * 2048;
   static constexpr int kBytes = kOperands + kGroups * NT * 8 * 8;
+  static constexpr int kPerStage = NT == 2 ? 2 : 1;  // units per stage of the ring of a
+  static constexpr int kStages = NT == 8 ? 3 : 4;
+  static constexpr int kWeightStages = NT == 8 ? 3 : 4;
+  static constexpr int kWarpBytes = kWeightStages * kStageBytes;
 };
 
 HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -130,12 +132,6 @@ HX_DEVICE float ld_cluster_f32(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
-}
-HX_DEVICE uint4 ld_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 HX_DEVICE void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -190,34 +186,52 @@ __global__ void __launch_bounds__(256) stage_kernel(const Args p, uint8_t* __res
   }
 }
 
-// One unit of a lane: the words of rows g and g + 8 and their groups' scales.
-template <typename T, int G>
-struct Unit {
-  uint32_t w[2][4];
-  T s[2][kUnitK / G];
-};
-
+// Adds one unit of a pair to the totals: w the warp's stage of weights (16 rows of 128 bytes, the 16-byte
+// chunks of row r permuted by r % 8), scales in the lane's s (groups 4 q + t of the pair in s[row][q],
+// handed round by shuffles).
 template <typename T, int G, int NT>
-HX_DEVICE void multiply(const Unit<T, G>& x, const uint8_t* block, float (&tot)[NT][4]) {
-  const int lane = threadIdx.x & 31, t = lane & 3;
+HX_DEVICE void multiply(const uint8_t* w, int unit, const float (&s)[2][kPair * (kUnitK / G) > 4 ? 2 : 1],
+                        const uint8_t* block, float (&tot)[NT][4]) {
+  constexpr int GU = kUnitK / G;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  uint32_t x[2][4];
 #pragma unroll
-  for (int j = 0; j < kUnitK / G; ++j) {
+  for (int r = 0; r < 2; ++r) {
+    const uint8_t* row = w + (g + 8 * r) * 128;
+    auto chunk = [&](int c) { return row + ((4 * unit + c) ^ g) * 16; };
+    if constexpr (G == 128) {
+      const uint4 v = *reinterpret_cast<const uint4*>(chunk(t));
+      x[r][0] = v.x, x[r][1] = v.y, x[r][2] = v.z, x[r][3] = v.w;
+    } else if constexpr (G == 64) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint2 v = *reinterpret_cast<const uint2*>(chunk(2 * j + (t >> 1)) + (t & 1) * 8);
+        x[r][2 * j] = v.x, x[r][2 * j + 1] = v.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[r][j] = *reinterpret_cast<const uint32_t*>(chunk(j) + 4 * t);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < GU; ++j) {
     float acc[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int y = 0; y < 4; ++y) acc[nt][y] = 0.f;
 #pragma unroll
-    for (int w = j * (G / 32); w < (j + 1) * (G / 32); ++w) {
-      const uint32_t x0 = x.w[0][w], y0 = x.w[1][w], x1 = x0 >> 8, y1 = y0 >> 8;
+    for (int i = j * (G / 32); i < (j + 1) * (G / 32); ++i) {
+      const uint32_t x0 = x[0][i], y0 = x[1][i], x1 = x0 >> 8, y1 = y0 >> 8;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const uint4 v = *reinterpret_cast<const uint4*>(block + (nt * 4 + w) * 512 + lane * 16);
+        const uint4 v = *reinterpret_cast<const uint4*>(block + (nt * 4 + i) * 512 + lane * 16);
         mma_f16(acc[nt], x0 & 0x000f000fu, y0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x00f000f0u, v.x, v.y);
         mma_f16(acc[nt], x1 & 0x000f000fu, y1 & 0x000f000fu, x1 & 0x00f000f0u, y1 & 0x00f000f0u, v.z, v.w);
       }
     }
-    const float s0 = DT<T>::to_f(x.s[0][j]) * 1048576.f, s1 = DT<T>::to_f(x.s[1][j]) * 1048576.f;
+    const int grp = unit * GU + j, from = (lane & ~3) | (grp & 3);
+    const float s0 = __shfl_sync(0xffffffffu, s[0][grp >> 2], from), s1 = __shfl_sync(0xffffffffu, s[1][grp >> 2], from);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const float4 f = *reinterpret_cast<const float4*>(block + Block<G, NT>::kOperands +
@@ -232,34 +246,58 @@ HX_DEVICE void multiply(const Unit<T, G>& x, const uint8_t* block, float (&tot)[
 
 template <typename T, int G, int NT, int EPI>
 __global__ void __launch_bounds__(kMaxWarps * 32, 2) gemm_q4_mma_kernel(
-    const Args p, const uint8_t* __restrict__ blocks, int S, int warps) {
+    const Args p, const __grid_constant__ CUtensorMap w_map, const uint8_t* __restrict__ blocks, int S,
+    int warps) {
   using B = Block<G, NT>;
   constexpr bool kRing = NT > 1;
-  constexpr int kPerStage = B::kPerStage, kAhead = B::kAhead;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[kStages], empty[kStages];
+  constexpr int kPerStage = B::kPerStage, kStages = B::kStages, kW = B::kWeightStages;
+  constexpr int kPairGroups = kPair * B::kGroups, kScales = kPairGroups > 4 ? 2 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  __shared__ uint64_t full[kStages], empty[kStages], w_full[kMaxWarps][kW];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  if (kRing) {
-    if (tid == 0) {
+  uint8_t* ring = smem + warp * B::kWarpBytes;
+  uint8_t* sm_a = smem + warps * B::kWarpBytes;
+  if (lane == 0) {
+    for (int i = 0; i < kW; ++i) mbar_init(&w_full[warp][i], 1);
+    if (kRing && warp == 0)
       for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], warps);
-      fence_mbar_init();
-    }
-    __syncthreads();
+    fence_mbar_init();
   }
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
   const int rank = S > 1 ? (int)cluster_rank() : 0;
   const int rows = warps * 16, n0 = (int)(blockIdx.x / S) * rows;
-  const int units = (p.K + kUnitK - 1) / kUnitK;
+  const int units = (p.K + kUnitK - 1) / kUnitK, groups = p.K / G;
   const int begin = (int)((int64_t)units * rank / S), end = (int)((int64_t)units * (rank + 1) / S);
-  float tot[NT][4];
+  const int pairs = (end - begin + kPair - 1) / kPair;
+  bool ok = true;
+
+  // Weights, 16 rows of two units: TMA fills rows past N and bytes past K with zeros.
+  const int w_at = begin * (kUnitK / 4), w_rows = n0 + warp * 16;  // in 16-bit elements
+  auto ask_weights = [&](int pair, int st) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&w_full[warp][st], kStageBytes);
+      tma_load_2d(ring + st * kStageBytes, &w_map, &w_full[warp][st], w_at + pair * (kPair * kUnitK / 4), w_rows);
+    }
+  };
+  for (int i = 0; i < min(pairs, kW); ++i) ask_weights(i, i);
+
+  // Scales of rows g and g + 8: lane t holds groups t and t + 4 of a pair, times 2^20.
+  const T* s_row[2] = {(const T*)p.scales + (int64_t)min(n0 + warp * 16 + g, p.N - 1) * groups,
+                       (const T*)p.scales + (int64_t)min(n0 + warp * 16 + g + 8, p.N - 1) * groups};
+  T next[2][kScales];
+  auto ask_scales = [&](int pair) {
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) tot[nt][j] = 0.f;
+      for (int q = 0; q < kScales; ++q)
+        next[r][q] = __ldg(s_row[r] + min((begin + pair * kPair) * B::kGroups + 4 * q + (t & (kPairGroups - 1)), groups - 1));
+  };
+  ask_scales(0);
 
   // Warp 0's lane 0: the next stage of a's blocks, once every warp has left the stage it replaces.
-  bool ok = true;
   int asked = 0;
   auto ask = [&]() {
     const int u = begin + asked * kPerStage, st = asked % kStages;
@@ -267,82 +305,66 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) gemm_q4_mma_kernel(
     if (asked >= kStages && !(ok = mbar_wait(&empty[st], (asked / kStages - 1) & 1))) return;
     const uint32_t bytes = (uint32_t)min(kPerStage, end - u) * B::kBytes;
     mbar_arrive_expect_tx(&full[st], bytes);
-    bulk_load(smem + st * (kPerStage * B::kBytes), blocks + (int64_t)u * B::kBytes, bytes, &full[st]);
+    bulk_load(sm_a + st * (kPerStage * B::kBytes), blocks + (int64_t)u * B::kBytes, bytes, &full[st]);
     ++asked;
   };
   if (kRing && tid == 0)
     for (int i = 0; i < kStages - 1; ++i) ask();
-  {
-    // Rows past N read row N - 1 and are not stored; groups past K (units are whole) read the last one
-    // and meet zeros of a.
-    const int groups = p.K / G, row0 = min(n0 + warp * 16 + g, p.N - 1), row1 = min(n0 + warp * 16 + g + 8, p.N - 1);
-    const uint8_t* wp[2] = {p.w + (int64_t)row0 * (p.K / 2) + t * (G / 8), p.w + (int64_t)row1 * (p.K / 2) + t * (G / 8)};
-    const T* sp[2] = {(const T*)p.scales + (int64_t)row0 * groups, (const T*)p.scales + (int64_t)row1 * groups};
-    using U = Unit<T, G>;
-    auto fetch = [&](U& x, int u) {
-      u = min(u, end - 1);
+
+  float tot[NT][4];
 #pragma unroll
-      for (int j = 0; j < B::kGroups; ++j) {
-        const int grp = G == 128 ? u : min(u * B::kGroups + j, groups - 1);
+  for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint8_t* at = wp[r] + grp * (G / 2);
-          if constexpr (G == 128) {
-            const uint4 v = ld_stream(at);
-            x.w[r][0] = v.x, x.w[r][1] = v.y, x.w[r][2] = v.z, x.w[r][3] = v.w;
-          } else if constexpr (G == 64) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
-            x.w[r][2 * j] = v.x, x.w[r][2 * j + 1] = v.y;
-          } else {
-            x.w[r][j] = __ldg(reinterpret_cast<const uint32_t*>(at));
-          }
-          x.s[r][j] = __ldg(sp[r] + grp);
-        }
+    for (int j = 0; j < 4; ++j) tot[nt][j] = 0.f;
+  int st = 0, phase = 0, w_st = 0, w_phase = 0, done = 0;
+  for (; done < pairs; ++done) {
+    const int u0 = begin + done * kPair;
+    if (!kRing && done % (kChunk / kPair) == 0) {  // stage a's slice: 16 bytes a thread, neighbours along k
+      __syncthreads();
+      const int per_row = min(kChunk, end - u0) * 16, items = p.M * per_row;
+      for (int i0 = 0; i0 < items; i0 += warps * 32) {
+        const int i = i0 + tid, m = min(i / per_row, p.M - 1), c = i - i / per_row * per_row;
+        const int64_t k = (int64_t)u0 * kUnitK + c * 8;
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (i < items && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)m * p.lda + k);
+        stage<T, G, NT>(sm_a + (c >> 4) * B::kBytes, m, c & 15, raw, i < items);
       }
-    };
-    U buf[kAhead];
+      __syncthreads();
+    }
+    float s[2][kScales];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) fetch(buf[i], begin + i);
-    int st = 0, phase = 0;
-    for (int c0 = begin; c0 < end; c0 += kRing ? end - begin : kChunk) {
-      const int c1 = kRing ? end : min(end, c0 + kChunk);
-      if (!kRing) {  // stage a's slice: 16 bytes a thread, neighbouring threads along k
-        if (c0 != begin) __syncthreads();
-        const int per_row = (c1 - c0) * 16, items = p.M * per_row;
-        for (int i0 = 0; i0 < items; i0 += warps * 32) {
-          const int i = i0 + tid, m = min(i / per_row, p.M - 1), c = i - i / per_row * per_row;
-          const int64_t k = (int64_t)c0 * kUnitK + c * 8;
-          uint4 raw = make_uint4(0, 0, 0, 0);
-          if (i < items && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)m * p.lda + k);
-          stage<T, G, NT>(smem + (c >> 4) * B::kBytes, m, c & 15, raw, i < items);
-        }
-        __syncthreads();
+    for (int r = 0; r < 2; ++r)
+#pragma unroll
+      for (int q = 0; q < kScales; ++q) s[r][q] = DT<T>::to_f(next[r][q]) * 1048576.f;
+    if (done + 1 < pairs) ask_scales(done + 1);
+    if (ok) ok = mbar_wait_warp(&w_full[warp][w_st], w_phase);
+#pragma unroll
+    for (int i = 0; i < kPair; ++i) {
+      if (u0 + i >= end || !ok) break;
+      if (kRing && i % kPerStage == 0) {
+        if (tid == 0) ask();
+        ok = mbar_wait_warp(&full[st], phase) && __all_sync(0xffffffffu, ok);
+        if (!ok) break;
       }
-      for (int u = c0; u < c1 && ok; u += kAhead) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          if (u + i >= c1) break;
-          if (kRing && i % kPerStage == 0) {
-            if (tid == 0) ask();
-            ok = mbar_wait_warp(&full[st], phase) && __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-          }
-          const uint8_t* block = kRing ? smem + (st * kPerStage + i % kPerStage) * B::kBytes
-                                       : smem + (u + i - c0) * B::kBytes;
-          multiply<T, G, NT>(buf[i], block, tot);
-          fetch(buf[i], u + i + kAhead);
-          if (kRing && (i % kPerStage == kPerStage - 1 || u + i + 1 == end)) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[st]);
-            if (++st == kStages) st = 0, phase ^= 1;
-          }
-        }
+      const uint8_t* block = kRing ? sm_a + (st * kPerStage + i % kPerStage) * B::kBytes
+                                   : sm_a + ((done % (kChunk / kPair)) * kPair + i) * B::kBytes;
+      multiply<T, G, NT>(ring + w_st * kStageBytes, i, s, block, tot);
+      if (kRing && (i % kPerStage == kPerStage - 1 || u0 + i + 1 == end)) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+        if (++st == kStages) st = 0, phase ^= 1;
       }
     }
+    if (!ok && kRing) break;  // up to eight rows the block's barriers go on
+    __syncwarp();
+    if (ok && done + kW < pairs) ask_weights(done + kW, w_st);
+    if (ok && ++w_st == kW) w_st = 0, w_phase ^= 1;
   }
-
-  if (kRing && tid == 0 && !ok)  // a wait gave up: let the copies in flight land
-    for (int i = max(0, asked - kStages); i < asked; ++i) mbar_wait_drain(&full[i % kStages], (i / kStages) & 1);
+  if (!ok) {  // a wait gave up: let the copies in flight land
+    for (int i = 0; i < kW; ++i) mbar_wait_drain(&w_full[warp][i], i < w_st ? w_phase ^ 1 : w_phase);
+    if (kRing && tid == 0)
+      for (int i = max(0, asked - kStages); i < asked; ++i) mbar_wait_drain(&full[i % kStages], (i / kStages) & 1);
+  }
 
   // Partials [batch row][weight row] in shared memory, added up over the cluster.
   __syncthreads();
@@ -410,14 +432,18 @@ int launch_mma(const Args& p, uint8_t* blocks, cudaStream_t stream) {
                                   "gemm_q4 stage_kernel launch");
     if (s) return s;
   }
-  const size_t staged = NT > 1 ? (size_t)kStages * B::kPerStage * B::kBytes
-                               : (size_t)std::min(kChunk, ceil_div(units, pl.S)) * B::kBytes;
-  const size_t smem = std::max(staged, (size_t)NT * 8 * (pl.warps * 16 + 4) * sizeof(float));
+  const size_t staged = (size_t)pl.warps * B::kWarpBytes +
+                        (size_t)(NT > 1 ? B::kStages * B::kPerStage : std::min(kChunk, ceil_div(units, pl.S))) * B::kBytes;
+  const size_t smem = std::max(staged, (size_t)NT * 8 * (pl.warps * 16 + 4) * sizeof(float)) + 1024;  // + alignment
+  CUtensorMap w_map;  // [N, K / 2] bytes as 16-bit elements
+  const uint64_t dims[2] = {(uint64_t)p.K / 4, (uint64_t)p.N}, strides[1] = {(uint64_t)p.K / 2};
+  const uint32_t box[2] = {kPair * kUnitK / 4, 16};
+  if (const int s = make_tensor_map(&w_map, p.w, 2, dims, strides, box, HX_BF16)) return s;
   auto kern = gemm_q4_mma_kernel<T, G, NT, EPI>;
-  if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+  if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 114 * 1024);
   return hx::cuda_status(
       launch_ex(kern, dim3((unsigned)(ceil_div(p.N, pl.warps * 16) * pl.S)),
-                dim3((unsigned)(pl.warps * 32)), smem, stream, pl.S, p,
+                dim3((unsigned)(pl.warps * 32)), smem, stream, pl.S, p, w_map,
                 (const uint8_t*)blocks, pl.S, pl.warps),
       "gemm_q4_mma_kernel launch");
 }
