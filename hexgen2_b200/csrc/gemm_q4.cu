@@ -86,19 +86,25 @@ __global__ void __launch_bounds__(kThreads) gemm_q4_kernel(const Args p) {
 //     where the codes are not, so bf16 and f16 values down to 2^-24 of the unit's largest are exact
 //     (smaller ones to 2^-35 of it). The factor comes off with the group's scale.
 //   - A unit is 16 weight rows x 128 k. Nibbles 16 bits apart make one operand register, and the order of
-//     k inside a group is free, so a lane reads whole words of its two rows straight from global
-//   - a is staged in the order of the B operands (one 16-byte load feeds two mma) with its group
-//     sums and factors: by every CTA for its own slice up to eight rows; above, once by
-//     stage_kernel, and warp 0 keeps a ring of its blocks filled.
-//   - A CTA has `warps` warps of 16 weight rows. K is split over the S CTAs of a cluster; each leaves
-//     f32 partials in its shared memory and CTA s adds up rows s, s + S, ... of the batch in rank
-//     order, applies the epilogue and stores neighbouring outputs together.
+//     k inside a group is free, so a lane takes whole words of its two rows (16 bytes at groups of 128).
+//   - The weights are what has to move, so a stays: a CTA keeps up to 16 rows of a over up to 4096 k (8
+//     rows: 8192 k) in shared memory in operand order, and the weight rows stream past it. Its 16 warps
+//     are R row tiles x KW slices of k; each streams its slice of one tile after another, two units at
+//     a time, through a ring of its own by TMA, and the KW partials of a tile are added up in slice order
+//     through shared memory. More rows of a are more CTAs on the same weights (passes side by side,
+//     so that a tile comes from HBM once and from L2 for the others), more k further rounds, whose
+//     running sums wait in an f32 workspace.
+//   Against this, with a streamed through shared memory and K split over clusters: clusters of 2 and 3
+//   left SMs idle (the fullest had 1.6 times the average), and staging a in every CTA of 128 rows cost a
+//   third of the instructions. Weights by plain loads, eight rows to an instruction, kept L1's tags 75 %
+//   busy at a quarter of the memory's bandwidth; bulk copies of 128 bytes took about 20 cycles each.
 // ------------------------------------------------------------------------------------------
-constexpr int kMaxWarps = 8;
+constexpr int kWarps = 16;
+constexpr int kMmaThreads = kWarps * 32;
 constexpr int kUnitK = 128;
-constexpr int kPair = 2;     // units per stage of a warp's ring of weights
+constexpr int kPair = 2;                     // units per stage of a warp's ring: 16 rows of 128 bytes
 constexpr int kStageBytes = 16 * 128;
-constexpr int kChunk = 16;   // units of a staged at a time up to eight rows
+constexpr int kSmem = 226 * 1024;  // dynamic; the barriers are static
 
 // One unit of a: operands [NT][4 words][8 rows][4 lanes] x 16 bytes, then [groups][NT * 8] (offset, factor).
 template <int G, int NT>
@@ -106,10 +112,8 @@ struct Block {
   static constexpr int kGroups = kUnitK / G;
   static constexpr int kOperands = NT * 2048;
   static constexpr int kBytes = kOperands + kGroups * NT * 8 * 8;
-  static constexpr int kPerStage = NT == 2 ? 2 : 1;  // units per stage of the ring of a
-  static constexpr int kStages = NT == 8 ? 3 : 4;
-  static constexpr int kWeightStages = NT == 8 ? 3 : 4;
-  static constexpr int kWarpBytes = kWeightStages * kStageBytes;
+  static constexpr int kMaxUnits = 64 / NT;             // of a in shared memory at a time
+  static constexpr int kPartial = kWarps * NT * 8 * 16;  // floats
 };
 
 HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -119,30 +123,8 @@ HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-HX_DEVICE uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-HX_DEVICE void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-HX_DEVICE float ld_cluster_f32(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
-  return v;
-}
-HX_DEVICE void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_u32(smem_dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
 
-// Elements [8 c, 8 c + 8) of a unit of batch row m (`raw`, zeros where a has none) into its block.
+// Elements [8 c, 8 c + 8) of a unit of row m of a (`raw`, zeros where a has none) into its block.
 // Called by whole warps, the 16 lanes of a unit side by side; `live` lanes store.
 template <typename T, int G, int NT>
 HX_DEVICE void stage(uint8_t* block, int m, int c, uint4 raw, bool live) {
@@ -161,29 +143,14 @@ HX_DEVICE void stage(uint8_t* block, int m, int c, uint4 raw, bool live) {
   }
   if (!live) return;
   const int ex = max((int)((__float_as_uint(big) >> 23) & 0xff) - 127, -100);
-  const float f = __uint_as_float((uint32_t)(127 + 9 - ex) << 23);
+  const float f = __uint_as_float((uint32_t)(127 + 9 - ex) << 23), f16 = f * 16.f;
   const int at = 8 * c, j = at / G, rest = at % G, t = rest / (G / 4), w = j * (G / 32) + rest % (G / 4) / 8;
   *reinterpret_cast<uint4*>(block + (((m >> 3) * 4 + w) * 32 + (m & 7) * 4 + t) * 16) =
-      make_uint4(pack2<__half>(x[0] * f * 16.f, x[4] * f * 16.f), pack2<__half>(x[1] * f, x[5] * f),
-                 pack2<__half>(x[2] * f * 16.f, x[6] * f * 16.f), pack2<__half>(x[3] * f, x[7] * f));
+      make_uint4(pack2<__half>(x[0] * f16, x[4] * f16), pack2<__half>(x[1] * f, x[5] * f),
+                 pack2<__half>(x[2] * f16, x[6] * f16), pack2<__half>(x[3] * f, x[7] * f));
   if (rest == 0)  // (offset, factor) of acc * factor + offset, both times 2^-20
     *reinterpret_cast<float2*>(block + Block<G, NT>::kOperands + (j * NT * 8 + m) * 8) =
         make_float2(sum * (-8.f / 1048576.f), __uint_as_float((uint32_t)(127 - 9 + ex) << 23));
-}
-
-template <typename T, int G, int NT>
-__global__ void __launch_bounds__(256) stage_kernel(const Args p, uint8_t* __restrict__ blocks) {
-  pdl_wait();
-  pdl_trigger();
-  const int u = blockIdx.x, c = threadIdx.x & 15;
-  const int64_t k = (int64_t)u * kUnitK + c * 8;
-#pragma unroll
-  for (int m0 = 0; m0 < NT * 8; m0 += 16) {
-    const int m = m0 + (threadIdx.x >> 4);
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (m < p.M && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)m * p.lda + k);
-    stage<T, G, NT>(blocks + (int64_t)u * Block<G, NT>::kBytes, m, c, raw, true);
-  }
 }
 
 // Adds one unit of a pair to the totals: w the warp's stage of weights (16 rows of 128 bytes, the 16-byte
@@ -244,233 +211,217 @@ HX_DEVICE void multiply(const uint8_t* w, int unit, const float (&s)[2][kPair * 
   }
 }
 
+struct Plan {
+  int kw;      // slices of k
+  int passes;  // CTAs that share a tile, each with NT * 8 rows of a
+  int ctas;    // per pass
+  int rounds;  // over k, of `units` units each (the last may have fewer)
+  int units;
+  int stages;  // of a warp's ring
+};
+
 template <typename T, int G, int NT, int EPI>
-__global__ void __launch_bounds__(kMaxWarps * 32, 2) gemm_q4_mma_kernel(
-    const Args p, const __grid_constant__ CUtensorMap w_map, const uint8_t* __restrict__ blocks, int S,
-    int warps) {
+__global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
+    const Args p, const __grid_constant__ CUtensorMap w_map, const Plan pl, float* __restrict__ running) {
   using B = Block<G, NT>;
-  constexpr bool kRing = NT > 1;
-  constexpr int kPerStage = B::kPerStage, kStages = B::kStages, kW = B::kWeightStages;
-  constexpr int kPairGroups = kPair * B::kGroups, kScales = kPairGroups > 4 ? 2 : 1;
+  constexpr int kPairGroups = kPair * B::kGroups, kScales = kPairGroups > 4 ? 2 : 1, kMaxStages = 4;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  __shared__ uint64_t full[kStages], empty[kStages], w_full[kMaxWarps][kW];
+  __shared__ uint64_t full[kWarps][kMaxStages];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* ring = smem + warp * B::kWarpBytes;
-  uint8_t* sm_a = smem + warps * B::kWarpBytes;
+  uint8_t* ring = smem + warp * pl.stages * kStageBytes;
+  float* part = reinterpret_cast<float*>(smem + kWarps * pl.stages * kStageBytes);  // [kWarps][NT * 8][16]
+  uint8_t* sm_a = reinterpret_cast<uint8_t*>(part + B::kPartial);
   if (lane == 0) {
-    for (int i = 0; i < kW; ++i) mbar_init(&w_full[warp][i], 1);
-    if (kRing && warp == 0)
-      for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], warps);
+    for (int i = 0; i < pl.stages; ++i) mbar_init(&full[warp][i], 1);
     fence_mbar_init();
   }
-  __syncthreads();
+  __syncwarp();
   pdl_wait();
   pdl_trigger();
-  const int rank = S > 1 ? (int)cluster_rank() : 0;
-  const int rows = warps * 16, n0 = (int)(blockIdx.x / S) * rows;
-  const int units = (p.K + kUnitK - 1) / kUnitK, groups = p.K / G;
-  const int begin = (int)((int64_t)units * rank / S), end = (int)((int64_t)units * (rank + 1) / S);
-  const int pairs = (end - begin + kPair - 1) / kPair;
+  const int R = kWarps / pl.kw, r = warp / pl.kw, kw = warp - r * pl.kw;
+  const int pass = blockIdx.x % pl.passes, first = blockIdx.x / pl.passes;
+  const int m0 = pass * NT * 8, M = min(NT * 8, p.M - m0);
+  const int tiles = (p.N + 15) / 16, steps_all = (tiles + R - 1) / R;  // of R tiles
+  const int steps = first < steps_all ? (steps_all - first + pl.ctas - 1) / pl.ctas : 0;
+  const int all_units = (p.K + kUnitK - 1) / kUnitK, groups = p.K / G;
   bool ok = true;
+  int st = 0, phase = 0;
 
-  // Weights, 16 rows of two units: TMA fills rows past N and bytes past K with zeros.
-  const int w_at = begin * (kUnitK / 4), w_rows = n0 + warp * 16;  // in 16-bit elements
-  auto ask_weights = [&](int pair, int st) {
-    if (lane == 0) {
-      mbar_arrive_expect_tx(&w_full[warp][st], kStageBytes);
-      tma_load_2d(ring + st * kStageBytes, &w_map, &w_full[warp][st], w_at + pair * (kPair * kUnitK / 4), w_rows);
-    }
-  };
-  for (int i = 0; i < min(pairs, kW); ++i) ask_weights(i, i);
-
-  // Scales of rows g and g + 8: lane t holds groups t and t + 4 of a pair, times 2^20.
-  const T* s_row[2] = {(const T*)p.scales + (int64_t)min(n0 + warp * 16 + g, p.N - 1) * groups,
-                       (const T*)p.scales + (int64_t)min(n0 + warp * 16 + g + 8, p.N - 1) * groups};
-  T next[2][kScales];
-  auto ask_scales = [&](int pair) {
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int q = 0; q < kScales; ++q)
-        next[r][q] = __ldg(s_row[r] + min((begin + pair * kPair) * B::kGroups + 4 * q + (t & (kPairGroups - 1)), groups - 1));
-  };
-  ask_scales(0);
-
-  // Warp 0's lane 0: the next stage of a's blocks, once every warp has left the stage it replaces.
-  int asked = 0;
-  auto ask = [&]() {
-    const int u = begin + asked * kPerStage, st = asked % kStages;
-    if (u >= end || !ok) return;
-    if (asked >= kStages && !(ok = mbar_wait(&empty[st], (asked / kStages - 1) & 1))) return;
-    const uint32_t bytes = (uint32_t)min(kPerStage, end - u) * B::kBytes;
-    mbar_arrive_expect_tx(&full[st], bytes);
-    bulk_load(sm_a + st * (kPerStage * B::kBytes), blocks + (int64_t)u * B::kBytes, bytes, &full[st]);
-    ++asked;
-  };
-  if (kRing && tid == 0)
-    for (int i = 0; i < kStages - 1; ++i) ask();
-
-  float tot[NT][4];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) tot[nt][j] = 0.f;
-  int st = 0, phase = 0, w_st = 0, w_phase = 0, done = 0;
-  for (; done < pairs; ++done) {
-    const int u0 = begin + done * kPair;
-    if (!kRing && done % (kChunk / kPair) == 0) {  // stage a's slice: 16 bytes a thread, neighbours along k
-      __syncthreads();
-      const int per_row = min(kChunk, end - u0) * 16, items = p.M * per_row;
-      for (int i0 = 0; i0 < items; i0 += warps * 32) {
-        const int i = i0 + tid, m = min(i / per_row, p.M - 1), c = i - i / per_row * per_row;
-        const int64_t k = (int64_t)u0 * kUnitK + c * 8;
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (i < items && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)m * p.lda + k);
-        stage<T, G, NT>(sm_a + (c >> 4) * B::kBytes, m, c & 15, raw, i < items);
+  for (int round = 0; round < pl.rounds; ++round) {
+    const int u0 = round * pl.units, units = min(pl.units, all_units - u0), pairs = (units + 1) / 2;
+    const int begin = kw * pairs / pl.kw, mine = (kw + 1) * pairs / pl.kw - begin;  // pairs of this warp
+    // The warp's stages in order: pair after pair of its slice, tile after tile. TMA fills rows past N and
+    // bytes past K with zeros; a tile past the last is all zeros.
+    int ahead = 0, ahead_step = 0, ahead_pair = 0, ahead_st = st;
+    const int total = ok ? steps * mine : 0;
+    auto ask = [&]() {
+      if (ahead >= total) return;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[warp][ahead_st], kStageBytes);
+        tma_load_2d(ring + ahead_st * kStageBytes, &w_map, &full[warp][ahead_st],
+                    (u0 / kPair + begin + ahead_pair) * (kPair * kUnitK / 4),
+                    ((first + ahead_step * pl.ctas) * R + r) * 16);
       }
-      __syncthreads();
+      ++ahead;
+      if (++ahead_pair == mine) ahead_pair = 0, ++ahead_step;
+      if (++ahead_st == pl.stages) ahead_st = 0;
+    };
+    for (int i = 0; i < pl.stages; ++i) ask();
+
+    // This round's a: 16 bytes a thread, neighbouring threads along k.
+    const int per_row = units * 16, items = M * per_row;
+    for (int i0 = 0; i0 < items; i0 += kMmaThreads) {
+      const int i = i0 + tid, m = min(i / per_row, M - 1), c = i - i / per_row * per_row;
+      const int64_t k = (int64_t)u0 * kUnitK + c * 8;
+      uint4 raw = make_uint4(0, 0, 0, 0);
+      if (i < items && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)(m0 + m) * p.lda + k);
+      stage<T, G, NT>(sm_a + (c >> 4) * B::kBytes, m, c & 15, raw, i < items);
     }
-    float s[2][kScales];
+    __syncthreads();
+
+    // Scales of rows g and g + 8 of a tile: lane t holds groups t and t + 4 of a pair, times 2^20. Rows past
+    // N and groups past K read the last ones and meet zeros.
+    T next[2][kScales];
+    auto ask_scales = [&](int step, int pair) {
+      const int row = ((first + step * pl.ctas) * R + r) * 16 + g;
+      const int grp = (u0 + (begin + pair) * kPair) * B::kGroups + (t & (kPairGroups - 1));
 #pragma unroll
-    for (int r = 0; r < 2; ++r)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int q = 0; q < kScales; ++q) s[r][q] = DT<T>::to_f(next[r][q]) * 1048576.f;
-    if (done + 1 < pairs) ask_scales(done + 1);
-    if (ok) ok = mbar_wait_warp(&w_full[warp][w_st], w_phase);
+        for (int q = 0; q < kScales; ++q)
+          next[h][q] = __ldg((const T*)p.scales + (int64_t)min(row + 8 * h, p.N - 1) * groups + min(grp + 4 * q, groups - 1));
+    };
+    if (total > 0) ask_scales(0, 0);
+
+    for (int step = 0; step < steps; ++step) {
+      float tot[NT][4];
 #pragma unroll
-    for (int i = 0; i < kPair; ++i) {
-      if (u0 + i >= end || !ok) break;
-      if (kRing && i % kPerStage == 0) {
-        if (tid == 0) ask();
-        ok = mbar_wait_warp(&full[st], phase) && __all_sync(0xffffffffu, ok);
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tot[nt][j] = 0.f;
+      for (int pair = 0; pair < mine && ok; ++pair) {
+        float s[2][kScales];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < kScales; ++q) s[h][q] = DT<T>::to_f(next[h][q]) * 1048576.f;
+        if (pair + 1 < mine) ask_scales(step, pair + 1);
+        else if (step + 1 < steps) ask_scales(step + 1, 0);
+        ok = mbar_wait_warp(&full[warp][st], phase);
         if (!ok) break;
-      }
-      const uint8_t* block = kRing ? sm_a + (st * kPerStage + i % kPerStage) * B::kBytes
-                                   : sm_a + ((done % (kChunk / kPair)) * kPair + i) * B::kBytes;
-      multiply<T, G, NT>(ring + w_st * kStageBytes, i, s, block, tot);
-      if (kRing && (i % kPerStage == kPerStage - 1 || u0 + i + 1 == end)) {
+        const uint8_t* block = sm_a + (begin + pair) * kPair * B::kBytes;
+        multiply<T, G, NT>(ring + st * kStageBytes, 0, s, block, tot);
+        if ((begin + pair) * kPair + 1 < units)
+          multiply<T, G, NT>(ring + st * kStageBytes, 1, s, block + B::kBytes, tot);
+        if (++st == pl.stages) st = 0, phase ^= 1;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
-        if (++st == kStages) st = 0, phase ^= 1;
+        ask();
       }
-    }
-    if (!ok && kRing) break;  // up to eight rows the block's barriers go on
-    __syncwarp();
-    if (ok && done + kW < pairs) ask_weights(done + kW, w_st);
-    if (ok && ++w_st == kW) w_st = 0, w_phase ^= 1;
-  }
-  if (!ok) {  // a wait gave up: let the copies in flight land
-    for (int i = 0; i < kW; ++i) mbar_wait_drain(&w_full[warp][i], i < w_st ? w_phase ^ 1 : w_phase);
-    if (kRing && tid == 0)
-      for (int i = max(0, asked - kStages); i < asked; ++i) mbar_wait_drain(&full[i % kStages], (i / kStages) & 1);
-  }
-
-  // Partials [batch row][weight row] in shared memory, added up over the cluster.
-  __syncthreads();
-  float* part = reinterpret_cast<float*>(smem);
-  const int pitch = rows + 4;
+      // Partials [slice][row of a][weight row], added up in slice order.
+      float* mine_at = part + warp * (NT * 8 * 16);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      part[(nt * 8 + 2 * t + (j & 1)) * pitch + warp * 16 + g + 8 * (j >> 1)] = tot[nt][j];
-  if (S > 1) cluster_sync(); else __syncthreads();
-  const int width = EPI == HX_EPI_SWIGLU ? rows / 2 : rows;  // outputs of one batch row in this CTA
-  const int cols = EPI == HX_EPI_SWIGLU ? p.N / 2 : p.N, col0 = EPI == HX_EPI_SWIGLU ? n0 / 2 : n0;
-  auto total = [&](int m, int r) {
-    const float* at = part + m * pitch + r;
-    if (S == 1) return *at;
-    float v = 0.f;
-    for (int s = 0; s < S; ++s) v += ld_cluster_f32(smem_u32(at), s);
-    return v;
-  };
-  const int mine = (p.M - rank + S - 1) / S * width;  // rows rank, rank + S, ...
-  for (int i = tid; i < mine; i += blockDim.x) {
-    const int m = rank + S * (i / width), c = i % width;
-    if (col0 + c >= cols) continue;
-    float v;
-    if constexpr (EPI == HX_EPI_SWIGLU) {
-      const int r = (c / 16) * 32 + c % 16;
-      v = total(m, r) * silu_f(total(m, r + 16));
-    } else {
-      v = total(m, c);
-      if (EPI == HX_EPI_RESIDUAL) v += DT<T>::to_f(((const T*)p.residual)[(int64_t)m * p.ldr + col0 + c]);
+        for (int j = 0; j < 4; ++j) mine_at[(nt * 8 + 2 * t + (j & 1)) * 16 + g + 8 * (j >> 1)] = tot[nt][j];
+      __syncthreads();
+      const int n0 = (first + step * pl.ctas) * R * 16;
+      auto total_of = [&](int m, int row) {
+        const float* at = part + (row >> 4) * pl.kw * (NT * 8 * 16) + m * 16 + (row & 15);
+        float v = 0.f;
+        for (int i = 0; i < pl.kw; ++i) v += at[i * (NT * 8 * 16)];
+        if (pl.rounds > 1) {
+          float* keep = running + (int64_t)(m0 + m) * p.N + n0 + row;
+          if (round > 0) v += *keep;
+          if (round + 1 < pl.rounds) *keep = v;
+        }
+        return v;
+      };
+      const bool last = round + 1 == pl.rounds;
+      constexpr bool kGated = EPI == HX_EPI_SWIGLU;
+      const int width = kGated ? R * 8 : R * 16, col0 = kGated ? n0 / 2 : n0, cols = kGated ? p.N / 2 : p.N;
+      for (int i = tid; i < M * width; i += kMmaThreads) {
+        const int m = i / width, c = i - m * width;
+        if (col0 + c >= cols) continue;
+        float v;
+        if constexpr (kGated) {
+          const int row = (c / 16) * 32 + c % 16;
+          const float up = total_of(m, row), gate = total_of(m, row + 16);
+          v = up * silu_f(gate);
+        } else {
+          v = total_of(m, c);
+          if (EPI == HX_EPI_RESIDUAL && last)
+            v += DT<T>::to_f(((const T*)p.residual)[(int64_t)(m0 + m) * p.ldr + col0 + c]);
+        }
+        if (last) ((T*)p.out)[(int64_t)(m0 + m) * p.ldo + col0 + c] = DT<T>::from_f(v);
+      }
+      __syncthreads();
     }
-    ((T*)p.out)[(int64_t)m * p.ldo + col0 + c] = DT<T>::from_f(v);
+    if (!ok)  // a wait gave up: let the copies in flight land
+      for (int i = 0; i < pl.stages; ++i) mbar_wait_drain(&full[warp][i], i < st ? phase ^ 1 : phase);
   }
-  if (S > 1) cluster_sync();  // no CTA leaves while others read its partials
 }
 
-int tiles_of(int64_t m) { return m <= 8 ? 1 : m <= 16 ? 2 : m <= 32 ? 4 : 8; }
-
-// Warps per CTA and CTAs per cluster: the pair whose fullest SM has the least to do, a CTA counting
-// its 16-row tiles times its units of K plus what it takes to start and to store (about 16 of those).
-struct Plan {
-  int warps, S;
-};
-Plan plan(int64_t n, int64_t k, bool pairs) {
-  const int tiles = ceil_div(n, 16), units = ceil_div(k, kUnitK);
-  Plan best{kMaxWarps, 1};
-  int64_t least = INT64_MAX;
-  for (int warps = kMaxWarps; warps >= 4; warps -= pairs ? 2 : 1)
-    for (int S = 1; S <= 8 && (S == 1 || 2 * S <= units); ++S) {
-      const int64_t ctas = (int64_t)ceil_div(tiles, warps) * S;
-      const int64_t cost = ceil_div(ctas, 148) * ((int64_t)warps * ceil_div(units, S) + 16);
-      if (cost < least) least = cost, best = {warps, S};
-    }
-  return best;
+// The slices of k that leave the fullest CTA the least to do: a step costs its pairs per warp, and about
+// 0.6 of a pair for adding up and storing.
+template <int G, int NT>
+Plan plan(int64_t m, int64_t n, int64_t k, bool gated) {
+  using B = Block<G, NT>;
+  Plan pl;
+  const int units = ceil_div(k, kUnitK), tiles = ceil_div(n, 16);
+  pl.rounds = ceil_div(units, B::kMaxUnits);
+  pl.units = ceil_div(units, pl.rounds);
+  pl.units += pl.units & 1;  // rounds begin at whole pairs
+  pl.rounds = ceil_div(units, pl.units);
+  pl.passes = ceil_div(m, NT * 8);
+  const int ctas = 148 / pl.passes, pairs = (pl.units + 1) / 2;
+  double least = 1e30;
+  for (int kw = gated ? kWarps / 2 : kWarps; kw >= 1; kw /= 2) {
+    if (kw > pairs && kw > 1) continue;
+    const double cost = ceil_div(ceil_div(tiles, kWarps / kw), ctas) * (ceil_div(pairs, kw) + 0.6);
+    if (cost < least) least = cost, pl.kw = kw;
+  }
+  pl.ctas = std::min(ctas, ceil_div(tiles, kWarps / pl.kw));
+  const size_t rest = kSmem - 1024 - B::kPartial * sizeof(float) - (size_t)pl.units * B::kBytes;
+  pl.stages = (int)std::min<size_t>(4, rest / (kWarps * kStageBytes));
+  return pl;
 }
 
 template <typename T, int G, int NT, int EPI>
-int launch_mma(const Args& p, uint8_t* blocks, cudaStream_t stream) {
+int launch_mma(const Args& p, float* running, cudaStream_t stream) {
   using B = Block<G, NT>;
-  const Plan pl = plan(p.N, p.K, EPI == HX_EPI_SWIGLU);
-  const int units = ceil_div(p.K, kUnitK);
-  if (NT > 1) {
-    const int s = hx::cuda_status(launch_ex(stage_kernel<T, G, NT>, dim3((unsigned)units), dim3(256), 0, stream, 1, p, blocks),
-                                  "gemm_q4 stage_kernel launch");
-    if (s) return s;
-  }
-  const size_t staged = (size_t)pl.warps * B::kWarpBytes +
-                        (size_t)(NT > 1 ? B::kStages * B::kPerStage : std::min(kChunk, ceil_div(units, pl.S))) * B::kBytes;
-  const size_t smem = std::max(staged, (size_t)NT * 8 * (pl.warps * 16 + 4) * sizeof(float)) + 1024;  // + alignment
+  const Plan pl = plan<G, NT>(p.M, p.N, p.K, EPI == HX_EPI_SWIGLU);
+  const size_t smem = 1024 + (size_t)kWarps * pl.stages * kStageBytes + B::kPartial * sizeof(float) + (size_t)pl.units * B::kBytes;
   CUtensorMap w_map;  // [N, K / 2] bytes as 16-bit elements
   const uint64_t dims[2] = {(uint64_t)p.K / 4, (uint64_t)p.N}, strides[1] = {(uint64_t)p.K / 2};
   const uint32_t box[2] = {kPair * kUnitK / 4, 16};
   if (const int s = make_tensor_map(&w_map, p.w, 2, dims, strides, box, HX_BF16)) return s;
   auto kern = gemm_q4_mma_kernel<T, G, NT, EPI>;
-  if (smem > 48 * 1024) cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 114 * 1024);
-  return hx::cuda_status(
-      launch_ex(kern, dim3((unsigned)(ceil_div(p.N, pl.warps * 16) * pl.S)),
-                dim3((unsigned)(pl.warps * 32)), smem, stream, pl.S, p, w_map,
-                (const uint8_t*)blocks, pl.S, pl.warps),
-      "gemm_q4_mma_kernel launch");
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  return hx::cuda_status(launch_ex(kern, dim3((unsigned)(pl.passes * pl.ctas)), dim3(kMmaThreads), smem, stream, 1, p,
+                                   w_map, pl, running),
+                         "gemm_q4_mma_kernel launch");
 }
 
 template <typename T, int G, int NT>
-int launch_epilogue(const Args& p, int epilogue, uint8_t* blocks, cudaStream_t stream) {
-  return epilogue == HX_EPI_SWIGLU     ? launch_mma<T, G, NT, HX_EPI_SWIGLU>(p, blocks, stream)
-         : epilogue == HX_EPI_RESIDUAL ? launch_mma<T, G, NT, HX_EPI_RESIDUAL>(p, blocks, stream)
-                                       : launch_mma<T, G, NT, HX_EPI_NONE>(p, blocks, stream);
+int launch_epilogue(const Args& p, int epilogue, float* running, cudaStream_t stream) {
+  return epilogue == HX_EPI_SWIGLU     ? launch_mma<T, G, NT, HX_EPI_SWIGLU>(p, running, stream)
+         : epilogue == HX_EPI_RESIDUAL ? launch_mma<T, G, NT, HX_EPI_RESIDUAL>(p, running, stream)
+                                       : launch_mma<T, G, NT, HX_EPI_NONE>(p, running, stream);
 }
 
 template <typename T, int G>
-int launch_rows(const Args& p, int epilogue, uint8_t* blocks, cudaStream_t stream) {
-  switch (tiles_of(p.M)) {
-    case 1: return launch_epilogue<T, G, 1>(p, epilogue, blocks, stream);
-    case 2: return launch_epilogue<T, G, 2>(p, epilogue, blocks, stream);
-    case 4: return launch_epilogue<T, G, 4>(p, epilogue, blocks, stream);
-    default: return launch_epilogue<T, G, 8>(p, epilogue, blocks, stream);
-  }
+int launch_rows(const Args& p, int epilogue, float* running, cudaStream_t stream) {
+  return p.M <= 8 ? launch_epilogue<T, G, 1>(p, epilogue, running, stream)
+                  : launch_epilogue<T, G, 2>(p, epilogue, running, stream);
 }
 
 template <typename T>
-int launch(const Args& p, int epilogue, uint8_t* blocks, cudaStream_t stream) {
+int launch(const Args& p, int epilogue, float* running, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    return p.group == 128  ? launch_rows<T, 128>(p, epilogue, blocks, stream)
-           : p.group == 64 ? launch_rows<T, 64>(p, epilogue, blocks, stream)
-                           : launch_rows<T, 32>(p, epilogue, blocks, stream);
+    return p.group == 128  ? launch_rows<T, 128>(p, epilogue, running, stream)
+           : p.group == 64 ? launch_rows<T, 64>(p, epilogue, running, stream)
+                           : launch_rows<T, 32>(p, epilogue, running, stream);
   } else {
     const int64_t cols = epilogue == HX_EPI_SWIGLU ? p.N / 2 : p.N;
     const dim3 grid((unsigned)ceil_div(cols, kThreads / 32), (unsigned)ceil_div(p.M, MB));
@@ -484,10 +435,9 @@ int launch(const Args& p, int epilogue, uint8_t* blocks, cudaStream_t stream) {
 
 }  // namespace
 
-extern "C" size_t hx_gemm_q4_workspace(int64_t m, int64_t k, int64_t group, int dtype) {
-  if (m <= 8 || m > 64 || k <= 0 || group < 32 || group > kUnitK || dtype == HX_F32) return 0;
-  const size_t nt = (size_t)tiles_of(m);
-  return (size_t)ceil_div(k, kUnitK) * nt * (2048 + (size_t)(kUnitK / group) * 64);
+extern "C" size_t hx_gemm_q4_workspace(int64_t m, int64_t n, int64_t k, int dtype) {
+  if (m <= 0 || m > 64 || n <= 0 || dtype == HX_F32 || k <= (m <= 8 ? 64 : 32) * kUnitK) return 0;
+  return (size_t)m * n * sizeof(float);
 }
 
 extern "C" int hx_gemm_q4(const void* a, const void* w, const void* scales, void* c, int64_t m,
@@ -511,11 +461,11 @@ extern "C" int hx_gemm_q4(const void* a, const void* w, const void* scales, void
   HX_REQUIRE(ldc >= cols && (epilogue != HX_EPI_RESIDUAL || ld_residual >= cols),
              "hx_gemm_q4: bad output or residual stride");
   if (m == 0) return HX_OK;
-  const size_t need = hx_gemm_q4_workspace(m, k, group, dtype);
+  const size_t need = hx_gemm_q4_workspace(m, n, k, dtype);
   HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
              "hx_gemm_q4: workspace too small (%zu < %zu) or misaligned", workspace_bytes, need);
   const Args p{a, (const uint8_t*)w, scales, residual, c, lda, ld_residual, ldc,
                (int)m, (int)n, (int)k, (int)group};
-  HX_DISPATCH_DTYPE(dtype, T, return launch<T>(p, epilogue, (uint8_t*)workspace, (cudaStream_t)stream));
+  HX_DISPATCH_DTYPE(dtype, T, return launch<T>(p, epilogue, (float*)workspace, (cudaStream_t)stream));
   return HX_OK;
 }

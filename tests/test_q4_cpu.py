@@ -127,8 +127,8 @@ P = 1 << 20  # an aligned address that is never followed: every call below fails
     ("hx_gemm_q4", [P, P, P, P, 2, 32, 64, 32, 66, 32, 0, None, 0, P, 1 << 30, 1, None]),  # lda
     ("hx_gemm_q4", [P, P, P, P, 2, 32, 64, 32, 64, 31, 0, None, 0, P, 1 << 30, 1, None]),  # ldc
     ("hx_gemm_q4", [P + 4, P, P, P, 1, 32, 64, 32, 64, 32, 0, None, 0, P, 1 << 30, 0, None]),
-    ("hx_gemm_q4", [P, P, P, P, 9, 32, 64, 32, 64, 32, 0, None, 0, P, 16, 1, None]),  # workspace
-    ("hx_gemm_q4", [P, P, P, P, 9, 32, 64, 32, 64, 32, 0, None, 0, P + 8, 1 << 30, 1, None]),
+    ("hx_gemm_q4", [P, P, P, P, 9, 32, 4224, 32, 4224, 32, 0, None, 0, P, 16, 1, None]),  # workspace
+    ("hx_gemm_q4", [P, P, P, P, 9, 32, 4224, 32, 4224, 32, 0, None, 0, P + 8, 1 << 30, 1, None]),
     ("hx_token_logprobs", [P, 2, 8, 7, P, 0, P, None, None, None, 0, None]),  # ld
     ("hx_token_logprobs", [P, 2, 8, 8, P, 9, P, None, P, P, 0, None]),  # top_k > cols
     ("hx_token_logprobs", [P, 2, 80, 80, P, 33, P, None, P, P, 0, None]),  # top_k > 32
