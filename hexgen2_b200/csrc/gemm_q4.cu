@@ -124,100 +124,118 @@ HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Largest |x| of eight 16-bit floats, as its bits (NaN above infinity above the rest).
+HX_DEVICE uint32_t largest_bits(uint4 v) {
+  const uint32_t m = 0x7fff7fffu;
+  const uint32_t a = __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+  return max(a & 0xffffu, a >> 16);
+}
+
 // Elements [8 c, 8 c + 8) of a unit of row m of a (`raw`, zeros where a has none) into its block.
 // Called by whole warps, the 16 lanes of a unit side by side; `live` lanes store.
 template <typename T, int G, int NT>
 HX_DEVICE void stage(uint8_t* block, int m, int c, uint4 raw, bool live) {
   const T* e = reinterpret_cast<const T*>(&raw);
-  float x[8], sum = 0.f, big = 0.f;
+  float x[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = DT<T>::to_f(e[i]);
-    sum += x[i];
-    big = fmaxf(big, fabsf(x[i]));
-  }
+  for (int i = 0; i < 8; ++i) x[i] = DT<T>::to_f(e[i]);
+  float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+  uint32_t bits = largest_bits(raw);
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
     if (o < G / 8) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
   }
-  if (!live) return;
-  const int ex = max((int)((__float_as_uint(big) >> 23) & 0xff) - 127, -100);
-  const float f = __uint_as_float((uint32_t)(127 + 9 - ex) << 23), f16 = f * 16.f;
+  const float big = DT<T>::to_f(__builtin_bit_cast(T, (unsigned short)bits));
+  const int ex = max((int)(__float_as_uint(big) >> 23), 27);  // biased; at least 2^-100
+  const float f = __uint_as_float((uint32_t)(263 - ex) << 23), f16 = f * 16.f;
   const int at = 8 * c, j = at / G, rest = at % G, t = rest / (G / 4), w = j * (G / 32) + rest % (G / 4) / 8;
+  if (!live) return;
   *reinterpret_cast<uint4*>(block + (((m >> 3) * 4 + w) * 32 + (m & 7) * 4 + t) * 16) =
       make_uint4(pack2<__half>(x[0] * f16, x[4] * f16), pack2<__half>(x[1] * f, x[5] * f),
                  pack2<__half>(x[2] * f16, x[6] * f16), pack2<__half>(x[3] * f, x[7] * f));
   if (rest == 0)  // (offset, factor) of acc * factor + offset, both times 2^-20
     *reinterpret_cast<float2*>(block + Block<G, NT>::kOperands + (j * NT * 8 + m) * 8) =
-        make_float2(sum * (-8.f / 1048576.f), __uint_as_float((uint32_t)(127 - 9 + ex) << 23));
+        make_float2(sum * (-8.f / 1048576.f), __uint_as_float((uint32_t)(ex - 9) << 23));
 }
 
-// Adds one unit of a pair to the totals: w the warp's stage of weights (16 rows of 128 bytes, the 16-byte
+// Adds a pair of units to the totals: w the warp's stage of weights (16 rows of 128 bytes, the 16-byte
 // chunks of row r permuted by r % 8), scales in the lane's s (groups 4 q + t of the pair in s[row][q],
-// handed round by shuffles).
+// handed round by shuffles), block the two units of a. The units' sums run side by side: one chain of mma
+// would wait for itself.
 template <typename T, int G, int NT>
-HX_DEVICE void multiply(const uint8_t* w, int unit, const float (&s)[2][kPair * (kUnitK / G) > 4 ? 2 : 1],
+HX_DEVICE void multiply(const uint8_t* w, const float (&s)[2][kPair * (kUnitK / G) > 4 ? 2 : 1],
                         const uint8_t* block, float (&tot)[NT][4]) {
+  using B = Block<G, NT>;
   constexpr int GU = kUnitK / G;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  uint32_t x[2][4];
+  uint32_t x[kPair][2][4];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const uint8_t* row = w + (g + 8 * r) * 128;
-    auto chunk = [&](int c) { return row + ((4 * unit + c) ^ g) * 16; };
-    if constexpr (G == 128) {
-      const uint4 v = *reinterpret_cast<const uint4*>(chunk(t));
-      x[r][0] = v.x, x[r][1] = v.y, x[r][2] = v.z, x[r][3] = v.w;
-    } else if constexpr (G == 64) {
+  for (int u = 0; u < kPair; ++u)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint2 v = *reinterpret_cast<const uint2*>(chunk(2 * j + (t >> 1)) + (t & 1) * 8);
-        x[r][2 * j] = v.x, x[r][2 * j + 1] = v.y;
+    for (int r = 0; r < 2; ++r) {
+      const uint8_t* row = w + (g + 8 * r) * 128;
+      auto chunk = [&](int c) { return row + ((4 * u + c) ^ g) * 16; };
+      if constexpr (G == 128) {
+        const uint4 v = *reinterpret_cast<const uint4*>(chunk(t));
+        x[u][r][0] = v.x, x[u][r][1] = v.y, x[u][r][2] = v.z, x[u][r][3] = v.w;
+      } else if constexpr (G == 64) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint2 v = *reinterpret_cast<const uint2*>(chunk(2 * j + (t >> 1)) + (t & 1) * 8);
+          x[u][r][2 * j] = v.x, x[u][r][2 * j + 1] = v.y;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[u][r][j] = *reinterpret_cast<const uint32_t*>(chunk(j) + 4 * t);
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[r][j] = *reinterpret_cast<const uint32_t*>(chunk(j) + 4 * t);
     }
-  }
 #pragma unroll
   for (int j = 0; j < GU; ++j) {
-    float acc[NT][4];
+    float acc[kPair][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int u = 0; u < kPair; ++u)
 #pragma unroll
-      for (int y = 0; y < 4; ++y) acc[nt][y] = 0.f;
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int i = j * (G / 32); i < (j + 1) * (G / 32); ++i) {
-      const uint32_t x0 = x[0][i], y0 = x[1][i], x1 = x0 >> 8, y1 = y0 >> 8;
+        for (int y = 0; y < 4; ++y) acc[u][nt][y] = 0.f;
+#pragma unroll
+    for (int i = j * (G / 32); i < (j + 1) * (G / 32); ++i)
+#pragma unroll
+      for (int u = 0; u < kPair; ++u) {
+        const uint32_t x0 = x[u][0][i], y0 = x[u][1][i], x1 = x0 >> 8, y1 = y0 >> 8;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 v = *reinterpret_cast<const uint4*>(block + u * B::kBytes + (nt * 4 + i) * 512 + lane * 16);
+          mma_f16(acc[u][nt], x0 & 0x000f000fu, y0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x00f000f0u, v.x, v.y);
+          mma_f16(acc[u][nt], x1 & 0x000f000fu, y1 & 0x000f000fu, x1 & 0x00f000f0u, y1 & 0x00f000f0u, v.z, v.w);
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) {
+      const int grp = u * GU + j, from = (lane & ~3) | (grp & 3);
+      const float s0 = __shfl_sync(0xffffffffu, s[0][grp >> 2], from), s1 = __shfl_sync(0xffffffffu, s[1][grp >> 2], from);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const uint4 v = *reinterpret_cast<const uint4*>(block + (nt * 4 + i) * 512 + lane * 16);
-        mma_f16(acc[nt], x0 & 0x000f000fu, y0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x00f000f0u, v.x, v.y);
-        mma_f16(acc[nt], x1 & 0x000f000fu, y1 & 0x000f000fu, x1 & 0x00f000f0u, y1 & 0x00f000f0u, v.z, v.w);
+        const float4 f = *reinterpret_cast<const float4*>(block + u * B::kBytes + B::kOperands +
+                                                          (j * NT * 8 + nt * 8 + 2 * t) * 8);
+        tot[nt][0] = fmaf(s0, fmaf(acc[u][nt][0], f.y, f.x), tot[nt][0]);
+        tot[nt][1] = fmaf(s0, fmaf(acc[u][nt][1], f.w, f.z), tot[nt][1]);
+        tot[nt][2] = fmaf(s1, fmaf(acc[u][nt][2], f.y, f.x), tot[nt][2]);
+        tot[nt][3] = fmaf(s1, fmaf(acc[u][nt][3], f.w, f.z), tot[nt][3]);
       }
-    }
-    const int grp = unit * GU + j, from = (lane & ~3) | (grp & 3);
-    const float s0 = __shfl_sync(0xffffffffu, s[0][grp >> 2], from), s1 = __shfl_sync(0xffffffffu, s[1][grp >> 2], from);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const float4 f = *reinterpret_cast<const float4*>(block + Block<G, NT>::kOperands +
-                                                        (j * NT * 8 + nt * 8 + 2 * t) * 8);
-      tot[nt][0] = fmaf(s0, fmaf(acc[nt][0], f.y, f.x), tot[nt][0]);
-      tot[nt][1] = fmaf(s0, fmaf(acc[nt][1], f.w, f.z), tot[nt][1]);
-      tot[nt][2] = fmaf(s1, fmaf(acc[nt][2], f.y, f.x), tot[nt][2]);
-      tot[nt][3] = fmaf(s1, fmaf(acc[nt][3], f.w, f.z), tot[nt][3]);
     }
   }
 }
 
 struct Plan {
-  int kw;      // slices of k
+  int log_kw;  // of the slices of k
   int passes;  // CTAs that share a tile, each with NT * 8 rows of a
   int ctas;    // per pass
   int rounds;  // over k, of `units` units each (the last may have fewer)
   int units;
   int stages;  // of a warp's ring
+  int buffers;  // of partials, one or two
 };
 
 template <typename T, int G, int NT, int EPI>
@@ -231,7 +249,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* ring = smem + warp * pl.stages * kStageBytes;
   float* part = reinterpret_cast<float*>(smem + kWarps * pl.stages * kStageBytes);  // [kWarps][NT * 8][16]
-  uint8_t* sm_a = reinterpret_cast<uint8_t*>(part + B::kPartial);
+  uint8_t* sm_a = reinterpret_cast<uint8_t*>(part + pl.buffers * B::kPartial);
   if (lane == 0) {
     for (int i = 0; i < pl.stages; ++i) mbar_init(&full[warp][i], 1);
     fence_mbar_init();
@@ -239,60 +257,74 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
   __syncwarp();
   pdl_wait();
   pdl_trigger();
-  const int R = kWarps / pl.kw, r = warp / pl.kw, kw = warp - r * pl.kw;
+  const int log_r = 4 - pl.log_kw, R = 1 << log_r, r = warp >> pl.log_kw, kw = warp & ((1 << pl.log_kw) - 1);
   const int pass = blockIdx.x % pl.passes, first = blockIdx.x / pl.passes;
   const int m0 = pass * NT * 8, M = min(NT * 8, p.M - m0);
-  const int tiles = (p.N + 15) / 16, steps_all = (tiles + R - 1) / R;  // of R tiles
+  const int tiles = (p.N + 15) / 16, steps_all = (tiles + R - 1) >> log_r;  // of R tiles
   const int steps = first < steps_all ? (steps_all - first + pl.ctas - 1) / pl.ctas : 0;
   const int all_units = (p.K + kUnitK - 1) / kUnitK, groups = p.K / G;
   bool ok = true;
   int st = 0, phase = 0;
 
   for (int round = 0; round < pl.rounds; ++round) {
-    const int u0 = round * pl.units, units = min(pl.units, all_units - u0), pairs = (units + 1) / 2;
-    const int begin = kw * pairs / pl.kw, mine = (kw + 1) * pairs / pl.kw - begin;  // pairs of this warp
-    // The warp's stages in order: pair after pair of its slice, tile after tile. TMA fills rows past N and
-    // bytes past K with zeros; a tile past the last is all zeros.
-    int ahead = 0, ahead_step = 0, ahead_pair = 0, ahead_st = st;
-    const int total = ok ? steps * mine : 0;
-    auto ask = [&]() {
-      if (ahead >= total) return;
+    const int u0 = round * pl.units, pairs = (min(pl.units, all_units - u0) + 1) / 2;
+    const int begin = (kw * pairs) >> pl.log_kw, mine = (((kw + 1) * pairs) >> pl.log_kw) - begin;  // pairs of this warp
+    // The warp's stages in order: pair after pair of its slice, tile after tile; the next one goes where the
+    // last was read. TMA fills rows past N and bytes past K with zeros; a tile past the last is all zeros.
+    const int x_first = (u0 / kPair + begin) * (kPair * kUnitK / 4), x_last = x_first + (mine - 1) * (kPair * kUnitK / 4);
+    int left = ok ? steps * mine : 0, x = x_first, y = (first * R + r) * 16;
+    auto ask = [&](int slot) {
+      if (left <= 0) return;
+      --left;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&full[warp][ahead_st], kStageBytes);
-        tma_load_2d(ring + ahead_st * kStageBytes, &w_map, &full[warp][ahead_st],
-                    (u0 / kPair + begin + ahead_pair) * (kPair * kUnitK / 4),
-                    ((first + ahead_step * pl.ctas) * R + r) * 16);
+        mbar_arrive_expect_tx(&full[warp][slot], kStageBytes);
+        tma_load_2d(ring + slot * kStageBytes, &w_map, &full[warp][slot], x, y);
       }
-      ++ahead;
-      if (++ahead_pair == mine) ahead_pair = 0, ++ahead_step;
-      if (++ahead_st == pl.stages) ahead_st = 0;
+      const bool wrap = x == x_last;
+      x = wrap ? x_first : x + kPair * kUnitK / 4;
+      y += wrap ? pl.ctas * R * 16 : 0;
     };
-    for (int i = 0; i < pl.stages; ++i) ask();
+    for (int i = 0, slot = st; i < pl.stages; ++i, slot = slot + 1 == pl.stages ? 0 : slot + 1) ask(slot);
 
-    // This round's a: 16 bytes a thread, neighbouring threads along k.
-    const int per_row = units * 16, items = M * per_row;
-    for (int i0 = 0; i0 < items; i0 += kMmaThreads) {
-      const int i = i0 + tid, m = min(i / per_row, M - 1), c = i - i / per_row * per_row;
-      const int64_t k = (int64_t)u0 * kUnitK + c * 8;
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (i < items && k < p.K) raw = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)(m0 + m) * p.lda + k);
-      stage<T, G, NT>(sm_a + (c >> 4) * B::kBytes, m, c & 15, raw, i < items);
+    // This round's a, whole pairs: a half warp per unit and row, 16 bytes a lane.
+    const int units = pairs * kPair, log_units = 32 - __clz(units - 1), c = lane & 15;
+    for (int i0 = warp * 2 + (lane >> 4); i0 < M << log_units; i0 += kWarps * 2 * 4) {
+      uint4 raw[4];  // four loads in flight
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * kWarps * 2, u = i & ((1 << log_units) - 1), m = i >> log_units;
+        const int64_t k = (int64_t)(u0 + u) * kUnitK + c * 8;
+        raw[j] = make_uint4(0, 0, 0, 0);
+        if (m < M && u < units && k < p.K)
+          raw[j] = *reinterpret_cast<const uint4*>((const T*)p.a + (int64_t)(m0 + m) * p.lda + k);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = i0 + j * kWarps * 2, u = i & ((1 << log_units) - 1), m = i >> log_units;
+        stage<T, G, NT>(sm_a + u * B::kBytes, m, c, raw[j], m < M && u < units);
+      }
     }
     __syncthreads();
 
     // Scales of rows g and g + 8 of a tile: lane t holds groups t and t + 4 of a pair, times 2^20. Rows past
     // N and groups past K read the last ones and meet zeros.
+    const T* s_row[2];
     T next[2][kScales];
+    const int grp0 = (u0 + begin * kPair) * B::kGroups + (t & (kPairGroups - 1));
     auto ask_scales = [&](int step, int pair) {
-      const int row = ((first + step * pl.ctas) * R + r) * 16 + g;
-      const int grp = (u0 + (begin + pair) * kPair) * B::kGroups + (t & (kPairGroups - 1));
+      if (pair == 0) {
+        const int row = ((first + step * pl.ctas) * R + r) * 16 + g;
+        s_row[0] = (const T*)p.scales + (int64_t)min(row, p.N - 1) * groups;
+        s_row[1] = (const T*)p.scales + (int64_t)min(row + 8, p.N - 1) * groups;
+      }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int q = 0; q < kScales; ++q)
-          next[h][q] = __ldg((const T*)p.scales + (int64_t)min(row + 8 * h, p.N - 1) * groups + min(grp + 4 * q, groups - 1));
+      for (int q = 0; q < kScales; ++q) {
+        const int grp = min(grp0 + pair * kPairGroups + 4 * q, groups - 1);
+        next[0][q] = __ldg(s_row[0] + grp);
+        next[1][q] = __ldg(s_row[1] + grp);
+      }
     };
-    if (total > 0) ask_scales(0, 0);
+    if (mine > 0) ask_scales(0, 0);
 
     for (int step = 0; step < steps; ++step) {
       float tot[NT][4];
@@ -300,7 +332,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 4; ++j) tot[nt][j] = 0.f;
-      for (int pair = 0; pair < mine && ok; ++pair) {
+#pragma unroll 1
+      for (int pair = 0; pair < mine; ++pair) {
         float s[2][kScales];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -308,18 +341,17 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
           for (int q = 0; q < kScales; ++q) s[h][q] = DT<T>::to_f(next[h][q]) * 1048576.f;
         if (pair + 1 < mine) ask_scales(step, pair + 1);
         else if (step + 1 < steps) ask_scales(step + 1, 0);
-        ok = mbar_wait_warp(&full[warp][st], phase);
+        if (ok) ok = mbar_wait_warp(&full[warp][st], phase);
         if (!ok) break;
-        const uint8_t* block = sm_a + (begin + pair) * kPair * B::kBytes;
-        multiply<T, G, NT>(ring + st * kStageBytes, 0, s, block, tot);
-        if ((begin + pair) * kPair + 1 < units)
-          multiply<T, G, NT>(ring + st * kStageBytes, 1, s, block + B::kBytes, tot);
-        if (++st == pl.stages) st = 0, phase ^= 1;
+        multiply<T, G, NT>(ring + st * kStageBytes, s, sm_a + (begin + pair) * kPair * B::kBytes, tot);
         __syncwarp();
-        ask();
+        ask(st);
+        if (++st == pl.stages) st = 0, phase ^= 1;
       }
-      // Partials [slice][row of a][weight row], added up in slice order.
-      float* mine_at = part + warp * (NT * 8 * 16);
+      // Partials [slice][row of a][weight row], added up in slice order. With two buffers the threads that
+      // add up (others at every step) do so while the rest go on.
+      float* buffer = part + (step & (pl.buffers - 1)) * B::kPartial;
+      float* mine_at = buffer + warp * (NT * 8 * 16);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -327,9 +359,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
       __syncthreads();
       const int n0 = (first + step * pl.ctas) * R * 16;
       auto total_of = [&](int m, int row) {
-        const float* at = part + (row >> 4) * pl.kw * (NT * 8 * 16) + m * 16 + (row & 15);
+        const float* at = buffer + ((row >> 4) << pl.log_kw) * (NT * 8 * 16) + m * 16 + (row & 15);
         float v = 0.f;
-        for (int i = 0; i < pl.kw; ++i) v += at[i * (NT * 8 * 16)];
+#pragma unroll 4
+        for (int i = 0; i < 1 << pl.log_kw; ++i) v += at[i * (NT * 8 * 16)];
         if (pl.rounds > 1) {
           float* keep = running + (int64_t)(m0 + m) * p.N + n0 + row;
           if (round > 0) v += *keep;
@@ -339,24 +372,25 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
       };
       const bool last = round + 1 == pl.rounds;
       constexpr bool kGated = EPI == HX_EPI_SWIGLU;
-      const int width = kGated ? R * 8 : R * 16, col0 = kGated ? n0 / 2 : n0, cols = kGated ? p.N / 2 : p.N;
-      for (int i = tid; i < M * width; i += kMmaThreads) {
-        const int m = i / width, c = i - m * width;
+      const int log_width = log_r + (kGated ? 3 : 4), col0 = kGated ? n0 / 2 : n0, cols = kGated ? p.N / 2 : p.N;
+      const int turn = pl.buffers == 2 ? step * (kMmaThreads / 4) : 0;
+      for (int i = (tid + turn) & (kMmaThreads - 1); i < M << log_width; i += kMmaThreads) {
+        const int m = i >> log_width, c = i & ((1 << log_width) - 1);
         if (col0 + c >= cols) continue;
-        float v;
+        float v, add = 0.f;
+        if (EPI == HX_EPI_RESIDUAL && last) add = DT<T>::to_f(((const T*)p.residual)[(int64_t)(m0 + m) * p.ldr + col0 + c]);
         if constexpr (kGated) {
           const int row = (c / 16) * 32 + c % 16;
           const float up = total_of(m, row), gate = total_of(m, row + 16);
           v = up * silu_f(gate);
         } else {
-          v = total_of(m, c);
-          if (EPI == HX_EPI_RESIDUAL && last)
-            v += DT<T>::to_f(((const T*)p.residual)[(int64_t)(m0 + m) * p.ldr + col0 + c]);
+          v = total_of(m, c) + add;
         }
         if (last) ((T*)p.out)[(int64_t)(m0 + m) * p.ldo + col0 + c] = DT<T>::from_f(v);
       }
-      __syncthreads();
+      if (pl.buffers == 1) __syncthreads();
     }
+    __syncthreads();  // every sum is read before the next round
     if (!ok)  // a wait gave up: let the copies in flight land
       for (int i = 0; i < pl.stages; ++i) mbar_wait_drain(&full[warp][i], i < st ? phase ^ 1 : phase);
   }
@@ -376,14 +410,17 @@ Plan plan(int64_t m, int64_t n, int64_t k, bool gated) {
   pl.passes = ceil_div(m, NT * 8);
   const int ctas = 148 / pl.passes, pairs = (pl.units + 1) / 2;
   double least = 1e30;
-  for (int kw = gated ? kWarps / 2 : kWarps; kw >= 1; kw /= 2) {
+  for (int log_kw = gated ? 3 : 4; log_kw >= 0; --log_kw) {
+    const int kw = 1 << log_kw;
     if (kw > pairs && kw > 1) continue;
     const double cost = ceil_div(ceil_div(tiles, kWarps / kw), ctas) * (ceil_div(pairs, kw) + 0.6);
-    if (cost < least) least = cost, pl.kw = kw;
+    if (cost < least) least = cost, pl.log_kw = log_kw;
   }
-  pl.ctas = std::min(ctas, ceil_div(tiles, kWarps / pl.kw));
-  const size_t rest = kSmem - 1024 - B::kPartial * sizeof(float) - (size_t)pl.units * B::kBytes;
-  pl.stages = (int)std::min<size_t>(4, rest / (kWarps * kStageBytes));
+  pl.ctas = std::min(ctas, ceil_div(tiles, kWarps >> pl.log_kw));
+  // What a leaves of shared memory: a second buffer of partials where two stages stay, then up to four stages.
+  const int64_t rest = kSmem - 1024 - (int64_t)pl.units * B::kBytes, buffer = B::kPartial * sizeof(float);
+  pl.buffers = rest - 2 * buffer >= 2 * kWarps * kStageBytes ? 2 : 1;
+  pl.stages = (int)std::min<int64_t>(4, (rest - pl.buffers * buffer) / (kWarps * kStageBytes));
   return pl;
 }
 
@@ -391,7 +428,8 @@ template <typename T, int G, int NT, int EPI>
 int launch_mma(const Args& p, float* running, cudaStream_t stream) {
   using B = Block<G, NT>;
   const Plan pl = plan<G, NT>(p.M, p.N, p.K, EPI == HX_EPI_SWIGLU);
-  const size_t smem = 1024 + (size_t)kWarps * pl.stages * kStageBytes + B::kPartial * sizeof(float) + (size_t)pl.units * B::kBytes;
+  const size_t smem = 1024 + (size_t)kWarps * pl.stages * kStageBytes + pl.buffers * B::kPartial * sizeof(float) +
+                      (size_t)pl.units * B::kBytes;
   CUtensorMap w_map;  // [N, K / 2] bytes as 16-bit elements
   const uint64_t dims[2] = {(uint64_t)p.K / 4, (uint64_t)p.N}, strides[1] = {(uint64_t)p.K / 2};
   const uint32_t box[2] = {kPair * kUnitK / 4, 16};
