@@ -268,10 +268,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
 
   for (int round = 0; round < pl.rounds; ++round) {
     const int u0 = round * pl.units, pairs = (min(pl.units, all_units - u0) + 1) / 2;
-    const int begin = (kw * pairs) >> pl.log_kw, mine = (((kw + 1) * pairs) >> pl.log_kw) - begin;  // pairs of this warp
+    // This warp's pairs: kw, kw + KW, ...: the KW warps of a tile read neighbouring bytes of its rows at a time.
+    const int mine = (pairs - kw + (1 << pl.log_kw) - 1) >> pl.log_kw;
     // The warp's stages in order: pair after pair of its slice, tile after tile; the next one goes where the
     // last was read. TMA fills rows past N and bytes past K with zeros; a tile past the last is all zeros.
-    const int x_first = (u0 / kPair + begin) * (kPair * kUnitK / 4), x_last = x_first + (mine - 1) * (kPair * kUnitK / 4);
+    const int x_step = (kPair * kUnitK / 4) << pl.log_kw;
+    const int x_first = (u0 / kPair + kw) * (kPair * kUnitK / 4), x_last = x_first + (mine - 1) * x_step;
     int left = ok ? steps * mine : 0, x = x_first, y = (first * R + r) * 16;
     auto ask = [&](int slot) {
       if (left <= 0) return;
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
         tma_load_2d(ring + slot * kStageBytes, &w_map, &full[warp][slot], x, y);
       }
       const bool wrap = x == x_last;
-      x = wrap ? x_first : x + kPair * kUnitK / 4;
+      x = wrap ? x_first : x + x_step;
       y += wrap ? pl.ctas * R * 16 : 0;
     };
     for (int i = 0, slot = st; i < pl.stages; ++i, slot = slot + 1 == pl.stages ? 0 : slot + 1) ask(slot);
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
     // N and groups past K read the last ones and meet zeros.
     const T* s_row[2];
     T next[2][kScales];
-    const int grp0 = (u0 + begin * kPair) * B::kGroups + (t & (kPairGroups - 1));
+    const int grp0 = (u0 + kw * kPair) * B::kGroups + (t & (kPairGroups - 1));
     auto ask_scales = [&](int step, int pair) {
       if (pair == 0) {
         const int row = ((first + step * pl.ctas) * R + r) * 16 + g;
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
       }
 #pragma unroll
       for (int q = 0; q < kScales; ++q) {
-        const int grp = min(grp0 + pair * kPairGroups + 4 * q, groups - 1);
+        const int grp = min(grp0 + ((pair * kPairGroups) << pl.log_kw) + 4 * q, groups - 1);
         next[0][q] = __ldg(s_row[0] + grp);
         next[1][q] = __ldg(s_row[1] + grp);
       }
@@ -343,7 +345,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
         else if (step + 1 < steps) ask_scales(step + 1, 0);
         if (ok) ok = mbar_wait_warp(&full[warp][st], phase);
         if (!ok) break;
-        multiply<T, G, NT>(ring + st * kStageBytes, s, sm_a + (begin + pair) * kPair * B::kBytes, tot);
+        multiply<T, G, NT>(ring + st * kStageBytes, s, sm_a + (kw + (pair << pl.log_kw)) * (kPair * B::kBytes), tot);
         __syncwarp();
         ask(st);
         if (++st == pl.stages) st = 0, phase ^= 1;
