@@ -10,17 +10,19 @@
 // read a long row while the others wait); the CTAs' sums meet through distributed shared memory, in
 // rank order.
 //
-// The top list needs no second pass over the row. T, the top_k-th largest of the best keys of 64 groups
-// of threads, is no larger than the row's top_k-th largest key, since top_k groups have an element at or
-// above it. Only threads whose best is at least T can own listed elements; they read their own elements
-// again and collect those >= T, in practice few more than top_k. A candidate's place in the list is
+// The top list needs no second pass over the row. A thread knows its maximum and the 16 bytes that hold
+// it first, so its best key lies between (maximum, last index there) and (maximum, first index there).
+// T, the top_k-th largest of the lower ends of 64 groups of threads, is no larger than the row's
+// top_k-th largest key, since top_k groups have an element at or above it. Only threads whose upper end is
+// at least T can own listed elements; they read their own elements again and collect those >= T, in
+// practice few more than top_k. A candidate's place in the list is
 // the number of larger candidates. Rows whose candidates do not fit, and rows with NaN, take top_k
 // rounds of "largest key below the last" instead.
 #include "common.cuh"
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;  // few, so that rows overlap: a row's last steps keep one or two warps busy
 constexpr int kWarps = kThreads / 32;
 constexpr int kGroups = 64;       // of kThreads / kGroups adjacent threads
 constexpr int kMaxTop = 32;
@@ -78,42 +80,76 @@ HX_DEVICE Key peek(const Key* p, int rank, int C) {
 // |d| 2^-24 of itself.
 HX_DEVICE float exp_neg(float d) { return ex2_approx(d * 1.4426950408889634f); }
 
-// The calling thread's elements of row[begin, end), in rising order: single elements up to a 16-byte
-// boundary, vectors with four loads in flight, single elements again. f(x, index) takes an array.
-template <typename T, typename F>
-HX_DEVICE void for_each(const T* row, int64_t begin, int64_t end, F&& f) {
-  constexpr int V = 16 / sizeof(T);
-  const int64_t first = min(begin + (int64_t)((16 - ((uintptr_t)(row + begin) & 15)) & 15) / (int64_t)sizeof(T), end);
-  const int64_t nvec = (end - first) / V, tail = first + nvec * V;
-  if (begin + threadIdx.x < first) {
-    float x[1] = {DT<T>::to_f(row[begin + threadIdx.x])};
-    f(x, begin + threadIdx.x);
+// row[begin, end) as thread `tid` of kThreads sees it: an element up to a 16-byte boundary, vectors tid, tid +
+// kThreads, ... of 16 bytes, an element behind them.
+template <typename T>
+struct Slice {
+  static constexpr int V = 16 / sizeof(T);
+  const T* row;
+  int64_t begin, end, first, nvec;
+  HX_DEVICE Slice(const T* row, int64_t begin, int64_t end) : row(row), begin(begin), end(end) {
+    first = min(begin + (int64_t)((16 - ((uintptr_t)(row + begin) & 15)) & 15) / (int64_t)sizeof(T), end);
+    nvec = (end - first) / V;
   }
-  const uint4* v = reinterpret_cast<const uint4*>(row + first);
-  for (int64_t base = threadIdx.x; base < nvec; base += 4 * kThreads) {
-    uint4 raw[4];
+  HX_DEVICE int64_t tail() const { return first + nvec * V; }
+  HX_DEVICE uint4 load(int64_t v) const { return __ldg(reinterpret_cast<const uint4*>(row + first) + v); }
+  static HX_DEVICE void convert(uint4 raw, float (&x)[V]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (base + u * kThreads < nvec) raw[u] = __ldg(v + base + u * kThreads);
+    for (int j = 0; j < V; ++j) x[j] = DT<T>::to_f(reinterpret_cast<const T*>(&raw)[j]);
+  }
+  // Thread tid's elements in rising order, four loads in flight. f(x, index) takes one or four runs of
+  // neighbouring elements, run u beginning at index + u * kThreads * (its length).
+  template <typename F>
+  HX_DEVICE void walk(F&& f) const {
+    const int tid = threadIdx.x;
+    if (begin + tid < first) {
+      float x[1][1] = {{DT<T>::to_f(row[begin + tid])}};
+      f(x, begin + tid);
+    }
+    int64_t v = tid;
+    for (; v + 3 * kThreads < nvec; v += 4 * kThreads) {
+      uint4 raw[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (base + u * kThreads >= nvec) break;
-      const T* e = reinterpret_cast<const T*>(&raw[u]);
-      float x[V];
+      for (int u = 0; u < 4; ++u) raw[u] = load(v + u * kThreads);
+      float x[4][V];
 #pragma unroll
-      for (int j = 0; j < V; ++j) x[j] = DT<T>::to_f(e[j]);
-      f(x, first + (base + u * kThreads) * V);
+      for (int u = 0; u < 4; ++u) convert(raw[u], x[u]);
+      f(x, first + v * V);
+    }
+    uint4 raw[3];
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (v + u * kThreads < nvec) raw[u] = load(v + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < 3; ++u)
+      if (v + u * kThreads < nvec) {
+        float x[1][V];
+        convert(raw[u], x[0]);
+        f(x, first + (v + u * kThreads) * V);
+      }
+    if (tail() + tid < end) {
+      float x[1][1] = {{DT<T>::to_f(row[tail() + tid])}};
+      f(x, tail() + tid);
     }
   }
-  if (tail + threadIdx.x < end) {
-    float x[1] = {DT<T>::to_f(row[tail + threadIdx.x])};
-    f(x, tail + threadIdx.x);
+  // The elements of thread `owner`, shared out over the calling warp. f(x, index), one at a time.
+  template <typename F>
+  HX_DEVICE void walk_together(int owner, F&& f) const {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0 && begin + owner < first) f(DT<T>::to_f(row[begin + owner]), begin + owner);
+    for (int64_t v = owner + (int64_t)lane * kThreads; v < nvec; v += 32 * kThreads) {
+      float x[V];
+      convert(load(v), x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f(x[j], first + v * V + j);
+    }
+    if (lane == 0 && tail() + owner < end) f(DT<T>::to_f(row[tail() + owner]), tail() + owner);
   }
-}
+};
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(
-    const T* __restrict__ logits, int64_t cols, int64_t ld, const int64_t* __restrict__ tokens, int C,
+__global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(
+    const T* __restrict__ logits, int64_t cols, int64_t ld, const int64_t* __restrict__ tokens, int log_c,
     int top_k, float* __restrict__ logprobs, float* __restrict__ entropy,
     float* __restrict__ top_logprobs, int64_t* __restrict__ top_tokens) {
   __shared__ float sm_max[kWarps], sm_z[kWarps], sm_s[kWarps], sm_total[3];
@@ -123,35 +159,55 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
   pdl_trigger();
-  const int64_t r = blockIdx.x / C;
+  const int C = 1 << log_c;
+  const int64_t r = blockIdx.x >> log_c;
   const int rank = C > 1 ? (int)cluster_rank() : 0;
   const T* row = logits + r * ld;
-  const int64_t begin = cols * rank / C, end = cols * (rank + 1) / C;
+  const Slice<T> slice(row, (cols * rank) >> log_c, (cols * (rank + 1)) >> log_c);
+
+  // The given token's logit, asked for ahead of the row.
+  float given = NAN;
+  if (logprobs && rank == 0 && tid == 0) {
+    const int64_t at = tokens[r];
+    if (at >= 0 && at < cols) given = DT<T>::to_f(row[at]);
+  }
 
   float m = -INFINITY, z = 0.f, s = 0.f;
-  int64_t where = -1;  // of the first element equal to m
-  for_each(row, begin, end, [&](auto& x, int64_t at) {
-    constexpr int n = sizeof(x) / sizeof(float);
-    float top = x[0];
+  int64_t where = -1;  // first index of the run that holds m first
+  int width = 0;       // and its length
+  slice.walk([&](auto& x, int64_t at) {
+    constexpr int U = sizeof(x) / sizeof(x[0]), V = sizeof(x[0]) / sizeof(float);
+    float tops[U], top = -INFINITY;
 #pragma unroll
-    for (int j = 1; j < n; ++j) top = fmaxf(top, x[j]);
-    if (where < 0) where = at;
+    for (int u = 0; u < U; ++u) {
+      tops[u] = x[u][0];
+#pragma unroll
+      for (int j = 1; j < V; ++j) tops[u] = fmaxf(tops[u], x[u][j]);
+      top = fmaxf(top, tops[u]);
+    }
+    if (where < 0) where = at, width = V;
     if (top > m) {
-      const float d = m - top, f = exp_neg(d);  // 0 and nothing to scale while m is -inf
-      if (m != -INFINITY) s = fmaf(d, z, s) * f, z *= f;
+      if (m != -INFINITY) {
+        const float d = m - top, f = exp_neg(d);
+        s = fmaf(d, z, s) * f;
+        z *= f;
+      }
       m = top;
-      int j = 0;
+      int at_u = 0;
 #pragma unroll
-      for (int i = n - 1; i >= 0; --i) j = x[i] == top ? i : j;
-      where = at + j;
+      for (int u = U - 1; u >= 0; --u) at_u = tops[u] == top ? u : at_u;
+      where = at + at_u * kThreads * V;
+      width = V;
     }
     const float ref = m == -INFINITY ? 0.f : m;  // masked logits alone so far: exp(-inf) = 0
 #pragma unroll
-    for (int j = 0; j < n; ++j) {
-      const float d = x[j] - ref, e = exp_neg(d);
-      z += e;
-      s = fmaf(e, fmaxf(d, -1000.f), s);  // 0 where d is -inf; a NaN stays in z
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = x[u][j] - ref, e = exp_neg(d);
+        z += e;
+        s = fmaf(e, fmaxf(d, -1000.f), s);  // 0 where d is -inf; a NaN stays in z
+      }
   });
 
   // The row's maximum, then the sums relative to it.
@@ -171,9 +227,9 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(
   s = warp_sum(s);
   if (lane == 0) sm_z[warp] = z, sm_s[warp] = s;
   // The best keys of the thread groups, for the top list.
-  const Key best = where >= 0 ? order_key(own, (uint32_t)where) : 0;
+  const Key most = where >= 0 ? order_key(own, (uint32_t)where) : 0;
   if (top_k > 0) {
-    Key k = best;
+    Key k = where >= 0 ? order_key(own, (uint32_t)(where + width - 1)) : 0;
 #pragma unroll
     for (int o = kThreads / kGroups / 2; o > 0; o >>= 1) {
       const Key other = __shfl_xor_sync(0xffffffffu, k, o);
@@ -193,27 +249,25 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(
   if (top_k > 0 && tid < kGroups) {  // this CTA's largest group keys, falling
     const Key mine = sm_group[tid];
     int place = 0;
-#pragma unroll 8
+#pragma unroll 16
     for (int i = 0; i < kGroups; ++i) place += sm_group[i] > mine;
     if (mine && place < top_k) sm_list[place] = mine;
   }
   if (C > 1) cluster_sync(); else __syncthreads();
-  top = -INFINITY;
-  for (int c = 0; c < C; ++c) top = fmaxf(top, peek(&sm_total[0], c, C));
-  z = s = 0.f;
-  for (int c = 0; c < C; ++c) {
-    const float mc = peek(&sm_total[0], c, C), zc = peek(&sm_total[1], c, C), sc = peek(&sm_total[2], c, C);
+  // The cluster's totals: lane c of every warp reads CTA c's.
+  {
+    const bool some = lane < C;
+    const float mc = some ? peek(&sm_total[0], lane, C) : -INFINITY;
+    const float zc = some ? peek(&sm_total[1], lane, C) : 0.f, sc = some ? peek(&sm_total[2], lane, C) : 0.f;
+    top = warp_max(mc);
     const float d = mc - top, f = mc == -INFINITY ? 1.f : exp_neg(d);  // without a maximum: 0, or NaN to keep
-    z += zc * f;
-    s += (mc == -INFINITY ? sc : fmaf(d, zc, sc)) * f;
+    z = warp_sum(zc * f);
+    s = warp_sum((mc == -INFINITY ? sc : fmaf(d, zc, sc)) * f);
   }
   if (top == -INFINITY) z = NAN;
   const float log_z = logf(z);
   if (rank == 0 && tid == 0) {
-    if (logprobs) {
-      const int64_t t = tokens[r];
-      logprobs[r] = t >= 0 && t < cols ? DT<T>::to_f(row[t]) - top - log_z : NAN;
-    }
+    if (logprobs) logprobs[r] = given - top - log_z;
     if (entropy) entropy[r] = log_z - s / z;
   }
   if (top_k == 0) {
@@ -227,41 +281,56 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(
   bool rounds = isnan(z);
   if (!rounds) {
     // T: the top_k-th largest of the CTAs' group keys (0, everything, where there are not as many).
-    for (int i = tid; i < C * top_k; i += kThreads) {
-      const Key mine = peek(&sm_list[i % top_k], i / top_k, C);
-      int place = 0;
-      for (int c = 0; c < C; ++c)
-        for (int j = 0; j < top_k; ++j) place += peek(&sm_list[j], c, C) > mine;
-      if (mine && place == top_k - 1) sm_limit = mine;
+    Key limit = sm_list[top_k - 1];
+    if (C > 1) {
+      const int n = C * top_k;
+      for (int i = tid; i < n; i += kThreads) sm_cand[i] = peek(&sm_list[i % top_k], i / top_k, C);
+      __syncthreads();
+      for (int i = tid; i < n; i += kThreads) {
+        const Key mine = sm_cand[i];
+        int place = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) place += sm_cand[j] > mine;
+        if (mine && place == top_k - 1) sm_limit = mine;
+      }
+      __syncthreads();  // sm_cand is free again
+      limit = sm_limit;
     }
-    __syncthreads();
-    const Key limit = sm_limit;
-    if (top_k == 1) {
-      if (rank == 0 && tid == 0) put(0, limit);
-    } else {
-      if (best >= limit && best)
-        for_each(row, begin, end, [&](auto& x, int64_t at) {
-          constexpr int n = sizeof(x) / sizeof(float);
-#pragma unroll
-          for (int j = 0; j < n; ++j) {
-            const Key k = order_key(x[j], (uint32_t)(at + j));
-            if (k >= limit) {
-              const int i = atomicAdd(&sm_count, 1);
-              if (i < kCandidates) sm_cand[i] = k;
-            }
-          }
-        });
-      if (C > 1) cluster_sync(); else __syncthreads();
-      for (int c = 0; c < C; ++c) rounds |= peek(&sm_count, c, C) > kCandidates;
+    const float least = limit ? key_value(limit) : -INFINITY;
+    // A warp walks the elements of its owning lanes together.
+    uint32_t owners = __ballot_sync(0xffffffffu, most >= limit && most);
+    while (owners) {
+      const int owner = (tid & ~31) + __ffs(owners) - 1;
+      owners &= owners - 1;
+      slice.walk_together(owner, [&](float x, int64_t at) {
+        if (x >= least) {
+          const Key k = order_key(x, (uint32_t)at);
+          const int i = k >= limit ? atomicAdd(&sm_count, 1) : kCandidates;
+          if (i < kCandidates) sm_cand[i] = k;
+        }
+      });
+    }
+    if (C > 1) cluster_sync(); else __syncthreads();
+    if (rank == 0) {  // the candidates of all CTAs, behind this one's
+      int n = sm_count;
+      if (C > 1) {
+        const int theirs = lane < C ? peek(&sm_count, lane, C) : 0;
+        for (int c = 1; c < C; ++c) {
+          const int k = __shfl_sync(0xffffffffu, theirs, c);
+          if (n <= kCandidates && n + k <= kCandidates)
+            for (int i = tid; i < k; i += kThreads) sm_cand[n + i] = peek(&sm_cand[i], c, C);
+          n += k;
+        }
+        __syncthreads();
+      }
+      rounds = n > kCandidates;
       if (!rounds)
-        for (int i = tid; i < sm_count; i += kThreads) {
-          const Key mine = sm_cand[i];
+        for (int i = tid; i < n; i += kThreads) {
+          const Key here = sm_cand[i];
           int place = 0;
-          for (int c = 0; c < C && place < top_k; ++c) {
-            const int n = peek(&sm_count, c, C);
-            for (int j = 0; j < n; ++j) place += peek(&sm_cand[j], c, C) > mine;
-          }
-          if (place < top_k) put(place, mine);
+#pragma unroll 8
+          for (int j = 0; j < n; ++j) place += sm_cand[j] > here;
+          if (place < top_k) put(place, here);
         }
     }
   }
@@ -303,14 +372,13 @@ extern "C" int hx_token_logprobs(const void* logits, int64_t rows, int64_t cols,
              (long long)top_k, kMaxTop);
   HX_REQUIRE(top_k == 0 || (top_logprobs && top_tokens), "hx_token_logprobs: no room for the top list");
   if (rows == 0) return HX_OK;
-  // CTAs per row: while all of them find room at once (four to an SM) and each keeps a thread's four
-  // loads in flight busy.
-  int C = 1;
-  while (C < 8 && rows * C * 2 <= 148 * 4 && cols / (C * 2) >= 4096) C *= 2;
+  // CTAs per row: while each keeps a thread's four loads in flight busy, as long as all find room at once.
+  int log_c = 0;
+  while (log_c < 3 && rows << (log_c + 1) <= 148 * 8 && cols >> (log_c + 1) >= 2048) ++log_c;
   HX_DISPATCH_DTYPE(dtype, T, {
     const int s = hx::cuda_status(
-        launch_ex(logprobs_kernel<T>, dim3((unsigned)(rows * C)), dim3(kThreads), 0, (cudaStream_t)stream,
-                  C, (const T*)logits, cols, ld, tokens, C, (int)top_k, logprobs, entropy,
+        launch_ex(logprobs_kernel<T>, dim3((unsigned)(rows << log_c)), dim3(kThreads), 0, (cudaStream_t)stream,
+                  1 << log_c, (const T*)logits, cols, ld, tokens, log_c, (int)top_k, logprobs, entropy,
                   top_logprobs, top_tokens),
         "logprobs_kernel launch");
     if (s) return s;
