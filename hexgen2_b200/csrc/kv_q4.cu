@@ -23,20 +23,18 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int E = 8;  // row elements per thread: 16 bytes of 16-bit input, one 32-bit word of codes
 
-template <typename T> HX_DEVICE void load8(const T* p, float (&x)[E]) {
-  if constexpr (sizeof(T) == 2) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&raw);
+// Eight row elements as they lie in memory.
+template <typename T> struct Raw {
+  uint4 v[sizeof(T) / 2];
+  HX_DEVICE void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = DT<T>::to_f(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p + i);
-      x[i] = v.x, x[i + 1] = v.y, x[i + 2] = v.z, x[i + 3] = v.w;
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = *(reinterpret_cast<const uint4*>(p) + i);
   }
-}
+  HX_DEVICE void to_f(float (&x)[E]) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = DT<T>::to_f(reinterpret_cast<const T*>(v)[i]);
+  }
+};
 
 template <typename T> HX_DEVICE void store8(T* p, const float (&x)[E]) {
   if constexpr (sizeof(T) == 2) {
@@ -52,106 +50,163 @@ template <typename T> HX_DEVICE void store8(T* p, const float (&x)[E]) {
   }
 }
 
+HX_DEVICE float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// Minimum and maximum of a row held by U adjacent lanes, NaN in both if there is one. 16-bit rows go as
+// packed pairs, the maximum as the negated minimum of the negated row (both exact), one shuffle a step.
+template <typename T, int U> HX_DEVICE void row_range(const Raw<T>& raw, float& lo, float& hi) {
+  if constexpr (sizeof(T) == 2) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* e = reinterpret_cast<const T2*>(raw.v);
+    const T2 least = __hmin2_nan(__hmin2_nan(e[0], e[1]), __hmin2_nan(e[2], e[3]));
+    const T2 most = __hmax2_nan(__hmax2_nan(e[0], e[1]), __hmax2_nan(e[2], e[3]));
+    T2 p;
+    p.x = __hmin_nan(least.x, least.y);
+    p.y = __hneg(__hmax_nan(most.x, most.y));
+#pragma unroll
+    for (int o = U / 2; o > 0; o >>= 1) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&p), o);
+      p = __hmin2_nan(p, *reinterpret_cast<const T2*>(&other));
+    }
+    lo = DT<T>::to_f(p.x);
+    hi = -DT<T>::to_f(p.y);
+  } else {
+    const float* e = reinterpret_cast<const float*>(raw.v);
+    float top = -e[0];
+    lo = e[0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) lo = min_nan(lo, e[i]), top = min_nan(top, -e[i]);
+#pragma unroll
+    for (int o = U / 2; o > 0; o >>= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      top = min_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    hi = -top;
+  }
+}
+
 // Encodes a row held by U adjacent lanes (E elements each; U a power of two, all lanes of the warp
 // call it) into its record: `half` 0 = K, 1 = V, `lane` the lane's place in the row.
-template <int U> HX_DEVICE void encode_row(const float (&x)[E], int lane, int half, bool live,
-                                          uint8_t* rec) {
+template <typename T, int U> HX_DEVICE void encode_row(const Raw<T>& raw, int lane, int half, bool live,
+                                                      uint8_t* rec) {
   constexpr int D = U * E;
-  float lo = x[0], hi = x[0], sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    sum += x[i] - x[i];  // NaN as soon as one element is not finite (fminf / fmaxf drop NaN)
-  }
-#pragma unroll
-  for (int o = U / 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  }
-  if (!live) return;
+  float lo, hi;
+  row_range<T, U>(raw, lo, hi);
   const float span = __fsub_rn(hi, lo);
   uint32_t word = 0;
   float scale = 0.f;
-  if (!(sum == 0.f) || isinf(span)) {
+  if (!(span < INFINITY)) {
     scale = lo = __int_as_float(0x7fffffff);
   } else if (span >= 7.888609052210118e-31f) {  // 2^-100
     scale = __fdiv_rn(span, 15.f);
     const float rate = __fdiv_rn(15.f, span);
+    float x[E];
+    raw.to_f(x);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int code = __float2int_rn(__fmul_rn(__fsub_rn(x[i], lo), rate));
-      word |= (uint32_t)min(code, 15) << (4 * i);
+      // Adding 1.5 * 2^23 leaves the nearest integer (ties to even) in the low bits; it is at most 15,
+      // span * rate being 15 up to two roundings.
+      const float y = __fadd_rn(__fmul_rn(__fsub_rn(x[i], lo), rate), 12582912.f);
+      word |= (__float_as_uint(y) & 15u) << (4 * i);
     }
   }
+  if (!live) return;
   *reinterpret_cast<uint32_t*>(rec + half * (D / 2) + lane * 4) = word;
   if (lane == 0) *reinterpret_cast<float2*>(rec + D + half * 8) = make_float2(scale, lo);
 }
 
-// Rows [0, counts[b]) of cache[b] -> records of cache_q4[b0 + b] at positions starts[b] + i.
-// U lanes per (row, K or V, head); heads fastest, so a warp reads consecutive bytes of one row.
+// Rows of a cache and positions of a 4-bit cache that belong together.
+struct Rows {
+  int64_t cbs, css;            // cache: elements per sequence and row
+  int64_t qbs, qhs, b0;        // 4-bit cache: bytes per sequence and head, first sequence
+  int64_t max_rows, max_seq;
+  const int32_t *starts, *counts;
+  int n_heads_kv, row_step;    // rows from one step of a unit to its next
+};
+
+// The range of sequence b: rows [0, n) and positions from `start`. Rows the buffers do not hold are not
+// touched; the caller learns of them.
+HX_DEVICE int64_t live_rows(const Rows& p, int b, int64_t& start) {
+  start = p.starts ? p.starts[b] : 0;
+  const int64_t want = p.counts[b], n = start < 0 ? 0 : min(want, min(p.max_rows, p.max_seq - start));
+  if ((want < 0 || start < 0 || n < want) && blockIdx.x == 0 && threadIdx.x == 0)
+    record_device_error(HX_DEVERR_BAD_ARGUMENT);
+  return n;
+}
+
+// cache -> records. A unit is U lanes on one (K or V, head), heads fastest, so a warp reads consecutive
+// bytes of a row; the grid is a whole number of rows, so a unit keeps its head from step to step.
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) quantize_kernel(
-    const T* __restrict__ cache, int64_t cbs, int64_t css, int64_t max_rows,
-    const int32_t* __restrict__ starts, const int32_t* __restrict__ counts, int n_heads_kv,
-    uint8_t* __restrict__ q4, int64_t qbs, int64_t qhs, int64_t b0, int64_t max_seq) {
-  constexpr int D = U * E, kUnits = kThreads / U;
+__global__ void __launch_bounds__(kThreads) quantize_kernel(const T* __restrict__ cache, uint8_t* __restrict__ q4,
+                                                           const Rows p) {
+  constexpr int D = U * E, kRec = D + 16;
   pdl_wait();
   pdl_trigger();
-  const int b = blockIdx.y;
-  const int64_t start = starts ? starts[b] : 0, want = counts[b];
-  // Rows the buffers do not hold are not touched; the caller learns of them.
-  const int64_t n = min(want, min(max_rows, max_seq - start));
-  if (want < 0 || start < 0 || n < want) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) record_device_error(HX_DEVERR_BAD_ARGUMENT);
-    if (start < 0) return;
-  }
-  const int lane = threadIdx.x % U;
-  const int64_t units = n * 2 * n_heads_kv;
-  for (int64_t base = (int64_t)blockIdx.x * kUnits; base < units; base += (int64_t)gridDim.x * kUnits) {
-    const int64_t unit = base + threadIdx.x / U;
-    const bool live = unit < units;
-    const int64_t row = live ? unit / (2 * n_heads_kv) : 0;
-    const int slot = live ? (int)(unit - row * (2 * n_heads_kv)) : 0;
-    const int half = slot >= n_heads_kv, head = slot - half * n_heads_kv;
-    float x[E];
-    load8(cache + b * cbs + row * css + (int64_t)slot * D + lane * E, x);
-    encode_row<U>(x, lane, half, live,
-                  q4 + (b0 + b) * qbs + head * qhs + (start + row) * (D + 16));
+  const int b = blockIdx.y, lane = threadIdx.x % U, slots = 2 * p.n_heads_kv;
+  int64_t start;
+  const int64_t n = live_rows(p, b, start);
+  const unsigned unit = blockIdx.x * (kThreads / U) + threadIdx.x / U;
+  int64_t row = unit / (unsigned)slots;
+  const int slot = (int)(unit - (unsigned)row * slots), half = slot >= p.n_heads_kv, head = slot - half * p.n_heads_kv;
+  const T* from = cache + b * p.cbs + row * p.css + slot * D + lane * E;
+  uint8_t* to = q4 + (p.b0 + b) * p.qbs + head * p.qhs + (start + row) * kRec;
+  const int64_t from_step = p.row_step * p.css;
+  // Lanes of a warp may be on different rows: it stays until all are done. Two loads in flight.
+  while (__any_sync(0xffffffffu, row < n)) {
+    Raw<T> raw[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (row + i * p.row_step < n) raw[i].load(from + i * from_step);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      encode_row<T, U>(raw[i], lane, half, row + i * p.row_step < n, to + (int64_t)i * p.row_step * kRec);
+    row += 2 * p.row_step;
+    from += 2 * from_step;
+    to += (int64_t)2 * p.row_step * kRec;
   }
 }
 
-// Records of cache_q4[b0 + b] at positions starts[b] + i -> rows [0, counts[b]) of cache[b].
+// records -> cache, by the same units.
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) dequantize_kernel(
-    const uint8_t* __restrict__ q4, int64_t qbs, int64_t qhs, int64_t b0, int64_t max_seq,
-    const int32_t* __restrict__ starts, const int32_t* __restrict__ counts, int n_heads_kv,
-    T* __restrict__ cache, int64_t cbs, int64_t css, int64_t max_rows) {
-  constexpr int D = U * E, kUnits = kThreads / U;
+__global__ void __launch_bounds__(kThreads) dequantize_kernel(const uint8_t* __restrict__ q4, T* __restrict__ cache,
+                                                             const Rows p) {
+  constexpr int D = U * E, kRec = D + 16;
   pdl_wait();
   pdl_trigger();
-  const int b = blockIdx.y;
-  const int64_t start = starts ? starts[b] : 0, want = counts[b];
-  const int64_t n = min(want, min(max_rows, max_seq - start));
-  if (want < 0 || start < 0 || n < want) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) record_device_error(HX_DEVERR_BAD_ARGUMENT);
-    if (start < 0) return;
-  }
-  const int lane = threadIdx.x % U;
-  const int64_t units = n * 2 * n_heads_kv;
-  for (int64_t unit = (int64_t)blockIdx.x * kUnits + threadIdx.x / U; unit < units;
-       unit += (int64_t)gridDim.x * kUnits) {
-    const int64_t row = unit / (2 * n_heads_kv);
-    const int slot = (int)(unit - row * (2 * n_heads_kv));
-    const int half = slot >= n_heads_kv, head = slot - half * n_heads_kv;
-    const uint8_t* rec = q4 + (b0 + b) * qbs + head * qhs + (start + row) * (D + 16);
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(rec + half * (D / 2) + lane * 4);
-    const float2 meta = *reinterpret_cast<const float2*>(rec + D + half * 8);
-    float x[E];
+  const int b = blockIdx.y, lane = threadIdx.x % U, slots = 2 * p.n_heads_kv;
+  int64_t start;
+  const int64_t n = live_rows(p, b, start);
+  const unsigned unit = blockIdx.x * (kThreads / U) + threadIdx.x / U;
+  int64_t row = unit / (unsigned)slots;
+  const int slot = (int)(unit - (unsigned)row * slots), half = slot >= p.n_heads_kv, head = slot - half * p.n_heads_kv;
+  const uint8_t* from = q4 + (p.b0 + b) * p.qbs + head * p.qhs + (start + row) * kRec + half * (D / 2) + lane * 4;
+  const int to_meta = D + half * 8 - half * (D / 2) - lane * 4;
+  T* to = cache + b * p.cbs + row * p.css + slot * D + lane * E;
+  const int64_t to_step = p.row_step * p.css, from_step = (int64_t)p.row_step * kRec;
+  for (; row < n; row += 2 * p.row_step, from += 2 * from_step, to += 2 * to_step) {
+    uint32_t word[2] = {};
+    float2 meta[2] = {};
 #pragma unroll
-    for (int i = 0; i < E; ++i) x[i] = fmaf(meta.x, (float)((word >> (4 * i)) & 15u), meta.y);
-    store8(cache + b * cbs + row * css + (int64_t)slot * D + lane * E, x);
+    for (int i = 0; i < 2; ++i)
+      if (row + i * p.row_step < n) {
+        word[i] = __ldg(reinterpret_cast<const uint32_t*>(from + i * from_step));
+        meta[i] = __ldg(reinterpret_cast<const float2*>(from + i * from_step + to_meta));
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (row + i * p.row_step >= n) break;
+      float x[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float code = __uint_as_float(((word[i] >> (4 * j)) & 15u) | 0x4b000000u) - 8388608.f;
+        x[j] = fmaf(meta[i].x, code, meta[i].y);
+      }
+      store8(to + i * to_step, x);
+    }
   }
 }
 
@@ -178,9 +233,11 @@ __global__ void __launch_bounds__(kThreads) rotary_q4_kernel(
   const bool live = at < units;
   const int unit = live ? at : units - 1;
   const T* src = qkv + token * units * D + (int64_t)unit * D;
-  float x[E];
-  load8(src + lane * E, x);
+  Raw<T> raw;
+  raw.load(src + lane * E);
   if (unit < n_heads + n_heads_kv) {
+    float x[E];
+    raw.to_f(x);
     const T* cs = cos_t + pos * (D / 2);
     const T* sn = sin_t + pos * (D / 2);
     if (kInterleaved) {
@@ -193,8 +250,10 @@ __global__ void __launch_bounds__(kThreads) rotary_q4_kernel(
       }
     } else {  // pairs (i, i + D/2): the partner chunk is U/2 lanes away
       const bool low = lane < U / 2;
+      Raw<T> partner;
+      partner.load(src + (low ? lane + U / 2 : lane - U / 2) * E);
       float y[E];
-      load8(src + (low ? lane + U / 2 : lane - U / 2) * E, y);
+      partner.to_f(y);
 #pragma unroll
       for (int i = 0; i < E; ++i) {
         const int f = (low ? lane : lane - U / 2) * E + i;
@@ -203,11 +262,12 @@ __global__ void __launch_bounds__(kThreads) rotary_q4_kernel(
                                : __fadd_rn(__fmul_rn(y[i], s), __fmul_rn(x[i], c)));
       }
     }
+    if (live && unit < n_heads) store8(q_out + (token * n_heads + unit) * D + lane * E, x);
+    store8(reinterpret_cast<T*>(raw.v), x);
   }
-  if (live && unit < n_heads) store8(q_out + (token * n_heads + unit) * D + lane * E, x);
   const int half = unit >= n_heads + n_heads_kv;
   const int head = unit - n_heads - half * n_heads_kv;
-  encode_row<U>(x, lane, half, live && unit >= n_heads,
+  encode_row<T, U>(raw, lane, half, live && unit >= n_heads,
                 q4 + (b0 + b) * qbs + head * qhs + pos * (D + 16));
 }
 
@@ -231,12 +291,18 @@ int check_rows(const char* who, const void* cache, int64_t cbs, int64_t css, int
   return HX_OK;
 }
 
-// CTAs per sequence: enough for every row the buffers can hold, at most a few waves in all (the
-// kernels stride over the live rows, which only the device knows).
-unsigned row_blocks(int64_t rows, int64_t batch, int64_t n_heads_kv, int U) {
-  const int64_t want = (rows * 2 * n_heads_kv * U + kThreads - 1) / kThreads;
+// CTAs per sequence: enough for two steps on every row the buffers can hold, at most a few waves in all
+// (the kernels stride over the live rows, which only the device knows), a whole number of rows.
+unsigned row_blocks(Rows& p, int64_t rows, int64_t batch, int U) {
+  const int64_t slots = 2 * p.n_heads_kv, units = kThreads / U;
+  int64_t whole = slots, rest = units;  // CTAs that make whole rows: slots / gcd(slots, units)
+  while (rest) std::swap(whole, rest), rest %= whole;
+  whole = slots / whole;
+  const int64_t want = (rows * slots + 2 * units - 1) / (2 * units);
   const int64_t cap = std::max<int64_t>(1, (int64_t)device_sm_count() * 32 / std::max<int64_t>(batch, 1));
-  return (unsigned)std::max<int64_t>(1, std::min(want, cap));
+  const int64_t blocks = (std::max<int64_t>(1, std::min(want, cap)) + whole - 1) / whole * whole;
+  p.row_step = (int)(blocks * units / slots);
+  return (unsigned)blocks;
 }
 
 }  // namespace
@@ -262,15 +328,15 @@ int hx_quantize_cache_q4(const void* cache, int64_t cache_batch_stride, int64_t 
   if (int s = check_rows("hx_quantize_cache_q4", cache, cache_batch_stride, cache_seq_stride,
                          n_heads_kv, head_dim, dtype))
     return s;
-  HX_REQUIRE(batch >= 0 && batch < 65536 && cache_rows >= 0, "hx_quantize_cache_q4: bad sizes");
+  HX_REQUIRE(batch >= 0 && batch < 65536 && cache_rows >= 0 && n_heads_kv < 32768, "hx_quantize_cache_q4: bad sizes");
   if (batch == 0 || cache_rows == 0) return HX_OK;
+  Rows p{cache_batch_stride, cache_seq_stride, q4_batch_stride, q4_head_stride, q4_batch_offset,
+         cache_rows, q4_max_seq, starts, counts, (int)n_heads_kv, 0};
   HX_DISPATCH_DTYPE(dtype, T, HX_Q4_DIM(head_dim, U, {
+    const unsigned blocks = row_blocks(p, cache_rows, batch, U);
     const int s = hx::cuda_status(
-        launch_ex(quantize_kernel<T, U>,
-                  dim3(row_blocks(cache_rows, batch, n_heads_kv, U), (unsigned)batch),
-                  dim3(kThreads), 0, (cudaStream_t)stream, 1, (const T*)cache, cache_batch_stride,
-                  cache_seq_stride, cache_rows, starts, counts, (int)n_heads_kv,
-                  (uint8_t*)cache_q4, q4_batch_stride, q4_head_stride, q4_batch_offset, q4_max_seq),
+        launch_ex(quantize_kernel<T, U>, dim3(blocks, (unsigned)batch), dim3(kThreads), 0,
+                  (cudaStream_t)stream, 1, (const T*)cache, (uint8_t*)cache_q4, p),
         "quantize_kernel launch");
     if (s) return s;
   }));
@@ -290,15 +356,15 @@ int hx_dequantize_cache_q4(const void* cache_q4, int64_t q4_batch_stride, int64_
   if (int s = check_rows("hx_dequantize_cache_q4", cache, cache_batch_stride, cache_seq_stride,
                          n_heads_kv, head_dim, dtype))
     return s;
-  HX_REQUIRE(batch >= 0 && batch < 65536 && cache_rows >= 0, "hx_dequantize_cache_q4: bad sizes");
+  HX_REQUIRE(batch >= 0 && batch < 65536 && cache_rows >= 0 && n_heads_kv < 32768, "hx_dequantize_cache_q4: bad sizes");
   if (batch == 0 || cache_rows == 0) return HX_OK;
+  Rows p{cache_batch_stride, cache_seq_stride, q4_batch_stride, q4_head_stride, q4_batch_offset,
+         cache_rows, q4_max_seq, starts, counts, (int)n_heads_kv, 0};
   HX_DISPATCH_DTYPE(dtype, T, HX_Q4_DIM(head_dim, U, {
+    const unsigned blocks = row_blocks(p, cache_rows, batch, U);
     const int s = hx::cuda_status(
-        launch_ex(dequantize_kernel<T, U>,
-                  dim3(row_blocks(cache_rows, batch, n_heads_kv, U), (unsigned)batch),
-                  dim3(kThreads), 0, (cudaStream_t)stream, 1, (const uint8_t*)cache_q4,
-                  q4_batch_stride, q4_head_stride, q4_batch_offset, q4_max_seq, starts, counts,
-                  (int)n_heads_kv, (T*)cache, cache_batch_stride, cache_seq_stride, cache_rows),
+        launch_ex(dequantize_kernel<T, U>, dim3(blocks, (unsigned)batch), dim3(kThreads), 0,
+                  (cudaStream_t)stream, 1, (const uint8_t*)cache_q4, (T*)cache, p),
         "dequantize_kernel launch");
     if (s) return s;
   }));
