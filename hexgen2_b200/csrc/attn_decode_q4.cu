@@ -592,8 +592,8 @@ int launch_mma(Args& a, int64_t batch, int64_t n_heads_kv, cudaStream_t stream) 
   a.q_chunks = ceil_div(a.group, NT * 4 * NJ);
   constexpr int smem = McSmem<D, NT>::kBytes;
   auto kern = decode_q4_mma_kernel<T, D, NT, NJ>;
-  if (smem > 48 * 1024)
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> allowed{0};  // devices where the kernel may use that much shared memory
+  if (const int s = allow_shared(reinterpret_cast<const void*>(kern), smem, allowed)) return s;
   const dim3 grid((unsigned)a.splits, (unsigned)(n_heads_kv * a.q_chunks), (unsigned)batch);
   return hx::cuda_status(launch_ex(kern, grid, dim3(kThreads), smem, stream, 1, a),
                          "decode_q4_mma_kernel launch");

@@ -14,6 +14,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -378,6 +379,19 @@ inline cudaError_t launch_ex(void (*kern)(KArgs...), dim3 grid, dim3 block, size
   cfg.attrs = attr;
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+
+// Host: lets `kern` use `bytes` of dynamic shared memory on the current device, asking the runtime once per
+// device (`allowed` is the kernel's own set of devices that know).
+inline int allow_shared(const void* kern, int bytes, std::atomic<uint64_t>& allowed) {
+  int dev = 0;
+  if (const int s = hx::cuda_status(cudaGetDevice(&dev), "cudaGetDevice")) return s;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return HX_OK;
+  const int s = hx::cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                                "cudaFuncSetAttribute");
+  if (s == HX_OK) allowed.fetch_or(bit, std::memory_order_relaxed);
+  return s;
 }
 
 // ---------------------------------------------------------------------------------------

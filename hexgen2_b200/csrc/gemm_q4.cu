@@ -437,7 +437,8 @@ int launch_mma(const Args& p, float* running, cudaStream_t stream) {
   const uint32_t box[2] = {kPair * kUnitK / 4, 16};
   if (const int s = make_tensor_map(&w_map, p.w, 2, dims, strides, box, HX_BF16)) return s;
   auto kern = gemm_q4_mma_kernel<T, G, NT, EPI>;
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<uint64_t> allowed{0};  // devices where the kernel may use that much shared memory
+  if (const int s = allow_shared(reinterpret_cast<const void*>(kern), kSmem, allowed)) return s;
   return hx::cuda_status(launch_ex(kern, dim3((unsigned)(pl.passes * pl.ctas)), dim3(kMmaThreads), smem, stream, 1, p,
                                    w_map, pl, running),
                          "gemm_q4_mma_kernel launch");

@@ -73,29 +73,33 @@ def workspace(nbytes: int, device=None, kind: str = "attn") -> torch.Tensor | No
     return buf
 
 
-def _device_of(*ts) -> int:
+def _device_of(first, *others) -> int:
     """The one CUDA device that all of the given tensors are on."""
-    dev = None
-    for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("hexgen2_b200 kernels take CUDA tensors (there is no CPU path)")
-        if dev is None:
-            dev = t.get_device()
-        elif t.get_device() != dev:
-            raise ValueError("all tensors of a call must be on the same device")
+    dev = first.get_device()  # -1 on the CPU
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            if dev >= 0 and t.is_cuda:
+                raise ValueError("all tensors of a call must be on the same device")
+            dev = -1
+    if dev < 0:
+        raise ValueError("hexgen2_b200 kernels take CUDA tensors (there is no CPU path)")
     return dev
 
 
-def _call(dev: int, name: str, *args):
-    """Calls entry point `name` with the current stream of device `dev`, whichever device is
-    current."""
+# The current stream of a device as an address, without making a Stream object (3 us of a call that takes
+# 10); and the device made current for a call whose tensors are elsewhere.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _call(dev: int, fn, *args):
+    """Calls a C entry point with the current stream of device `dev`, whichever device is current."""
     if dev == torch.cuda.current_device():
-        check(getattr(_L(), name)(*args, _stream()), name)
+        st = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            check(getattr(_L(), name)(*args, _stream()), name)
+            st = fn(*args, _raw_stream(dev))
+    if st:
+        check(st, fn.__name__)
 
 
 # ----------------------------------------------------------------------------- norms
@@ -364,7 +368,7 @@ def quantize_cache_q4(cache, counts, cache_q4, starts=None, batch_offset=0):
     dev = _device_of(cache, counts, cache_q4, starts)
     if cache.numel() == 0:
         return cache_q4
-    _call(dev, "hx_quantize_cache_q4", cache.data_ptr(), cache.stride(0), cache.stride(1),
+    _call(dev, _L().hx_quantize_cache_q4, cache.data_ptr(), cache.stride(0), cache.stride(1),
           cache.shape[1], _p(starts), counts.data_ptr(), B, hk, d, cache_q4.data_ptr(),
           cache_q4.stride(0), cache_q4.stride(1), batch_offset, cache_q4.shape[2], _code(cache))
     _count(1)
@@ -385,7 +389,7 @@ def dequantize_cache_q4(cache_q4, counts, cache, starts=None, batch_offset=0):
     dev = _device_of(cache, counts, cache_q4, starts)
     if cache.numel() == 0:
         return cache
-    _call(dev, "hx_dequantize_cache_q4", cache_q4.data_ptr(), cache_q4.stride(0),
+    _call(dev, _L().hx_dequantize_cache_q4, cache_q4.data_ptr(), cache_q4.stride(0),
           cache_q4.stride(1), batch_offset, cache_q4.shape[2], _p(starts), counts.data_ptr(), B, hk,
           d, cache.data_ptr(), cache.stride(0), cache.stride(1), cache.shape[1], _code(cache))
     _count(1)
@@ -413,7 +417,7 @@ def rotary_cache_write_q4(qkv, batch, seqlen, n_heads, n_heads_kv, head_dim, pos
         raise ValueError(f"{what}: q_out must be contiguous [batch, seqlen, n_heads, head_dim] in qkv's dtype")
     if qkv.numel() == 0:
         return q_out
-    _call(dev, "hx_rotary_cache_write_q4", qkv.data_ptr(), batch, seqlen, n_heads, n_heads_kv,
+    _call(dev, _L().hx_rotary_cache_write_q4, qkv.data_ptr(), batch, seqlen, n_heads, n_heads_kv,
           head_dim, pos_start.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
           1 if interleaved else 0, q_out.data_ptr(), cache_q4.data_ptr(), cache_q4.stride(0),
           cache_q4.stride(1), batch_offset, cache_q4.shape[2], _code(qkv))
@@ -442,7 +446,7 @@ def decode_attention_q4(q, cache_q4, seqlens, n_heads_kv, max_seqlen, softmax_sc
     nbytes = decode_q4_workspace_bytes(B, hq, n_heads_kv, d, max_seqlen)
     # A buffer of its own for every call: calls on several streams, and graphs, do not share it.
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _call(dev, "hx_decode_attention_q4", q.data_ptr(), q.stride(0), cache_q4.data_ptr(),
+    _call(dev, _L().hx_decode_attention_q4, q.data_ptr(), q.stride(0), cache_q4.data_ptr(),
           cache_q4.stride(0), cache_q4.stride(1), seqlens.data_ptr(), B, hq, n_heads_kv, d,
           max_seqlen, float(softmax_scale), out.data_ptr(), _p(ws), nbytes, _code(q))
     _count(2 if nbytes else 1)
@@ -485,7 +489,7 @@ def gemm_q4(a, w_q4, scales, epilogue=HX_EPI_NONE, residual=None, out=None):
     if K > 4096:  # a buffer of its own for every call, as in decode_attention_q4
         nbytes = _L().hx_gemm_q4_workspace(M, N, K, code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
-    _call(dev, "hx_gemm_q4", a.data_ptr(), w_q4.data_ptr(), scales.data_ptr(), out.data_ptr(), M, N,
+    _call(dev, _L().hx_gemm_q4, a.data_ptr(), w_q4.data_ptr(), scales.data_ptr(), out.data_ptr(), M, N,
           K, group, a.stride(0) if M > 1 else max(K, a.stride(0)),
           out.stride(0) if M > 1 else cols, epilogue, _p(residual),
           0 if residual is None else residual.stride(0) if M > 1 else cols, _p(ws), nbytes, code)
@@ -532,7 +536,7 @@ def token_logprobs(logits, tokens=None, top_k=0, entropy=False) -> TokenLogprobs
         ids = torch.empty(rows, top_k, dtype=torch.long, device=logits.device)
     if rows == 0:
         return TokenLogprobs(logp, ent, top, ids)
-    _call(dev, "hx_token_logprobs", logits.data_ptr(), rows, cols,
+    _call(dev, _L().hx_token_logprobs, logits.data_ptr(), rows, cols,
           logits.stride(0) if rows > 1 else max(cols, logits.stride(0)), _p(tokens), top_k, _p(logp),
           _p(ent), _p(top), _p(ids), _code(logits))
     _count(1)
