@@ -99,6 +99,9 @@ __global__ void __launch_bounds__(kThreads) gemm_q4_kernel(const Args p) {
 //   third of the instructions. Weights by plain loads, eight rows to an instruction, kept L1's tags 75 %
 //   busy at a quarter of the memory's bandwidth; bulk copies of 128 bytes took about 20 cycles each.
 // ------------------------------------------------------------------------------------------
+#ifndef HX_TC_MIN
+#define HX_TC_MIN 0
+#endif
 constexpr int kWarps = 16;
 constexpr int kMmaThreads = kWarps * 32;
 constexpr int kUnitK = 128;
@@ -131,15 +134,16 @@ HX_DEVICE uint32_t largest_bits(uint4 v) {
   return max(a & 0xffffu, a >> 16);
 }
 
-// Elements [8 c, 8 c + 8) of a unit of row m of a (`raw`, zeros where a has none) into its block.
-// Called by whole warps, the 16 lanes of a unit side by side; `live` lanes store.
-template <typename T, int G, int NT>
-HX_DEVICE void stage(uint8_t* block, int m, int c, uint4 raw, bool live) {
+// Eight elements of a row of a (`raw`; the 16 lanes of a unit of 128 k side by side, whole warps) as operands:
+// times the unit's power of two, in the order of the codes' pairs (0,4), (1,5), (2,6), (3,7), the even pairs
+// times 16. sum: of the group's elements (f32); factor: what brings a sum of products back, times 2^-20.
+template <typename T, int G>
+HX_DEVICE uint4 operands(uint4 raw, float& sum, float& factor) {
   const T* e = reinterpret_cast<const T*>(&raw);
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = DT<T>::to_f(e[i]);
-  float sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+  sum = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
   uint32_t bits = largest_bits(raw);
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) {
@@ -149,14 +153,22 @@ HX_DEVICE void stage(uint8_t* block, int m, int c, uint4 raw, bool live) {
   const float big = DT<T>::to_f(__builtin_bit_cast(T, (unsigned short)bits));
   const int ex = max((int)(__float_as_uint(big) >> 23), 27);  // biased; at least 2^-100
   const float f = __uint_as_float((uint32_t)(263 - ex) << 23), f16 = f * 16.f;
+  factor = __uint_as_float((uint32_t)(ex - 9) << 23);
+  return make_uint4(pack2<__half>(x[0] * f16, x[4] * f16), pack2<__half>(x[1] * f, x[5] * f),
+                    pack2<__half>(x[2] * f16, x[6] * f16), pack2<__half>(x[3] * f, x[7] * f));
+}
+
+// Elements [8 c, 8 c + 8) of a unit of row m of a (zeros where a has none) into its block; `live` lanes store.
+template <typename T, int G, int NT>
+HX_DEVICE void stage(uint8_t* block, int m, int c, uint4 raw, bool live) {
+  float sum, factor;
+  const uint4 op = operands<T, G>(raw, sum, factor);
   const int at = 8 * c, j = at / G, rest = at % G, t = rest / (G / 4), w = j * (G / 32) + rest % (G / 4) / 8;
   if (!live) return;
-  *reinterpret_cast<uint4*>(block + (((m >> 3) * 4 + w) * 32 + (m & 7) * 4 + t) * 16) =
-      make_uint4(pack2<__half>(x[0] * f16, x[4] * f16), pack2<__half>(x[1] * f, x[5] * f),
-                 pack2<__half>(x[2] * f16, x[6] * f16), pack2<__half>(x[3] * f, x[7] * f));
+  *reinterpret_cast<uint4*>(block + (((m >> 3) * 4 + w) * 32 + (m & 7) * 4 + t) * 16) = op;
   if (rest == 0)  // (offset, factor) of acc * factor + offset, both times 2^-20
     *reinterpret_cast<float2*>(block + Block<G, NT>::kOperands + (j * NT * 8 + m) * 8) =
-        make_float2(sum * (-8.f / 1048576.f), __uint_as_float((uint32_t)(ex - 9) << 23));
+        make_float2(sum * (-8.f / 1048576.f), factor);
 }
 
 // Adds a pair of units to the totals: w the warp's stage of weights (16 rows of 128 bytes, the 16-byte
@@ -227,6 +239,16 @@ HX_DEVICE void multiply(const uint8_t* w, const float (&s)[2][kPair * (kUnitK / 
     }
   }
 }
+
+HX_DEVICE void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+#include "gemm_q4_tc.cuh"
 
 struct Plan {
   int log_kw;  // of the slices of k
@@ -426,6 +448,9 @@ Plan plan(int64_t m, int64_t n, int64_t k, bool gated) {
   return pl;
 }
 
+// Whether the tcgen05 kernel takes a product.
+bool use_tc(int64_t m, int64_t n, int64_t k) { return m > 8 && n * k >= HX_TC_MIN; }
+
 template <typename T, int G, int NT, int EPI>
 int launch_mma(const Args& p, float* running, cudaStream_t stream) {
   using B = Block<G, NT>;
@@ -460,6 +485,10 @@ int launch_rows(const Args& p, int epilogue, float* running, cudaStream_t stream
 template <typename T>
 int launch(const Args& p, int epilogue, float* running, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
+    if (use_tc(p.M, p.N, p.K))
+      return p.group == 128  ? tc::launch_rows<T, 128>(p, epilogue, running, stream)
+             : p.group == 64 ? tc::launch_rows<T, 64>(p, epilogue, running, stream)
+                             : tc::launch_rows<T, 32>(p, epilogue, running, stream);
     return p.group == 128  ? launch_rows<T, 128>(p, epilogue, running, stream)
            : p.group == 64 ? launch_rows<T, 64>(p, epilogue, running, stream)
                            : launch_rows<T, 32>(p, epilogue, running, stream);
@@ -476,9 +505,10 @@ int launch(const Args& p, int epilogue, float* running, cudaStream_t stream) {
 
 }  // namespace
 
-extern "C" size_t hx_gemm_q4_workspace(int64_t m, int64_t n, int64_t k, int dtype) {
-  if (m <= 0 || m > 64 || n <= 0 || dtype == HX_F32 || k <= (m <= 8 ? 64 : 32) * kUnitK) return 0;
-  return (size_t)m * n * sizeof(float);
+extern "C" size_t hx_gemm_q4_workspace(int64_t m, int64_t n, int64_t k, int64_t group, int dtype) {
+  if (m <= 0 || m > 64 || n <= 0 || k <= 0 || group < 32 || group > kUnitK || dtype == HX_F32) return 0;
+  if (use_tc(m, n, k)) return tc::workspace(m, n, k, group);
+  return k <= (m <= 8 ? 64 : 32) * kUnitK ? 0 : (size_t)m * n * sizeof(float);
 }
 
 extern "C" int hx_gemm_q4(const void* a, const void* w, const void* scales, void* c, int64_t m,
@@ -502,7 +532,7 @@ extern "C" int hx_gemm_q4(const void* a, const void* w, const void* scales, void
   HX_REQUIRE(ldc >= cols && (epilogue != HX_EPI_RESIDUAL || ld_residual >= cols),
              "hx_gemm_q4: bad output or residual stride");
   if (m == 0) return HX_OK;
-  const size_t need = hx_gemm_q4_workspace(m, n, k, dtype);
+  const size_t need = hx_gemm_q4_workspace(m, n, k, group, dtype);
   HX_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (uintptr_t)workspace % 16 == 0),
              "hx_gemm_q4: workspace too small (%zu < %zu) or misaligned", workspace_bytes, need);
   const Args p{a, (const uint8_t*)w, scales, residual, c, lda, ld_residual, ldc,

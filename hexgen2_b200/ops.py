@@ -486,8 +486,8 @@ def gemm_q4(a, w_q4, scales, epilogue=HX_EPI_NONE, residual=None, out=None):
     if M == 0:
         return out
     group, code, nbytes, ws = K // scales.shape[1], _code(a), 0, None
-    if K > 4096:  # a buffer of its own for every call, as in decode_attention_q4
-        nbytes = _L().hx_gemm_q4_workspace(M, N, K, code)
+    if M > 8 or K > 4096:  # a buffer of its own for every call, as in decode_attention_q4
+        nbytes = _L().hx_gemm_q4_workspace(M, N, K, group, code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
     _call(dev, _L().hx_gemm_q4, a.data_ptr(), w_q4.data_ptr(), scales.data_ptr(), out.data_ptr(), M, N,
           K, group, a.stride(0) if M > 1 else max(K, a.stride(0)),

@@ -288,7 +288,7 @@ int hx_gemm_q4(const void* a, const void* w, const void* scales, void* c, int64_
                int64_t k, int64_t group, int64_t lda, int64_t ldc, int epilogue,
                const void* residual, int64_t ld_residual, void* workspace, size_t workspace_bytes,
                int dtype, void* stream);
-size_t hx_gemm_q4_workspace(int64_t m, int64_t n, int64_t k, int dtype);
+size_t hx_gemm_q4_workspace(int64_t m, int64_t n, int64_t k, int64_t group, int dtype);
 
 /* ---------------------------------------------------------------- sampling */
 /* out_idx[r] = first index of the maximum of logits[r, 0:cols] (torch.argmax semantics).
