@@ -22,7 +22,6 @@ constexpr int kThreads = 18 * 32;
 constexpr int kRows = 128;
 constexpr int kWeightBytes = kRows * 128;  // of an item: 256 k
 constexpr int kAccs = 4;                   // accumulators in flight
-constexpr uint32_t kAccColumn = 128;       // behind the two 64-column operands
 
 // An item of a: two units of swizzled operands ([2 halves of 64 k][NT rows][128 bytes]), then (offset, factor)
 // [2 units][groups][NT].
@@ -34,6 +33,10 @@ struct Item {
   static constexpr int kBytes = 2 * kUnit + kStats;
   static constexpr int kPitch = (kWeightBytes + kBytes + 1023) / 1024 * 1024;  // of the ring
   static constexpr int kStages = NT == 64 ? 4 : NT == 32 ? 6 : 8;
+  // Operands of 64 columns in tensor memory, half of them for either unit; the accumulators behind them.
+  // (With one per unit its way round, unpack - MMA - free, took 3000 cycles an item.)
+  static constexpr int kPer = NT == 64 ? 2 : 3;
+  static constexpr uint32_t kAccColumn = kPer * 2 * 64;
   static constexpr int kShared = kStages * kPitch + 1024;
 };
 
@@ -75,11 +78,11 @@ HX_DEVICE bool wait(uint64_t* bar, uint32_t parity) {
   bool done = mbar_try_wait(bar, parity);
   if (!done) {
     const unsigned long long t0 = globaltimer_ns();
-    while (!(done = mbar_try_wait(bar, parity)))
-      if (globaltimer_ns() - t0 > HX_WAIT_LIMIT_NS) {
-        record_device_error(HX_DEVERR_WAIT_TIMEOUT);
-        break;
-      }
+    do {  // the timer is far away: a look at it costs as much as a product of a unit
+#pragma unroll 1
+      for (int i = 0; i < 256 && !done; ++i) done = mbar_try_wait(bar, parity);
+    } while (!done && globaltimer_ns() - t0 <= HX_WAIT_LIMIT_NS);
+    if (!done) record_device_error(HX_DEVERR_WAIT_TIMEOUT);
   }
   return __all_sync(0xffffffffu, done);
 }
@@ -106,15 +109,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
     const Args p, const __grid_constant__ CUtensorMap w_map, const uint8_t* __restrict__ blocks,
     float* __restrict__ parts, int items_per_block, int total) {
   using I = Item<G, NT>;
-  constexpr int kStages = I::kStages, kHalf = NT / 2;
+  constexpr int kStages = I::kStages, kHalf = NT / 2, kPer = I::kPer;
+  constexpr uint32_t kAccColumn = I::kAccColumn;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  __shared__ uint64_t full[kStages], empty[kStages], a_full[2], a_empty[2], d_full[kAccs], d_empty[kAccs];
+  __shared__ uint64_t full[kStages], empty[kStages], a_full[2 * kPer], a_empty[2 * kPer], d_full[kAccs], d_empty[kAccs];
   __shared__ uint32_t tmem_at;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 17);
-    for (int i = 0; i < 2; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
+    for (int i = 0; i < 2 * kPer; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
     for (int i = 0; i < kAccs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 8);
     fence_mbar_init();
   }
@@ -150,40 +154,42 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
       for (int i = max(0, n - kStages); i < n; ++i) mbar_wait_drain(&full[i % kStages], (i / kStages) & 1);
   } else if (warp == 1) {
     constexpr uint32_t idesc = make_idesc_f16<__half>(128, NT);
-    int acc = 0, acc_phase = 0;
+    const uint64_t desc = sw128_kmajor_desc(smem_u32(smem + kWeightBytes));
+    int acc = 0, acc_phase = 0, st = 0, st_phase = 0, per = 0, per_phase = 0;
     for (int n = 0; n < end - begin && ok; ++n) {
-      const int st = n % kStages;
-      const uint32_t b = smem_u32(smem + st * I::kPitch + kWeightBytes);
-      if (!(ok = wait(&full[st], (n / kStages) & 1))) break;
-#pragma unroll 1
-      for (int u = 0; u < 2 && ok; ++u) {
-        if (!(ok = wait(&a_full[u], n & 1))) break;
+      if (!(ok = wait(&full[st], st_phase))) break;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (!(ok = wait(&a_full[2 * per + u], per_phase))) break;
         tc_fence_after();
-#pragma unroll 1
+#pragma unroll
         for (int j = 0; j < I::kGroups; ++j) {
           if (!(ok = wait(&d_empty[acc], acc_phase ^ 1))) break;
           tc_fence_after();
           if (lane == 0) {
+            const uint64_t b = desc + ((st * I::kPitch + u * I::kUnit) >> 4);
+            const uint32_t d = tmem + kAccColumn + acc * NT, from = tmem + (2 * per + u) * 64;
 #pragma unroll
             for (int i = 0; i < G / 16; ++i) {
               const int k = j * (G / 16) + i;  // 16 k at a time: 8 columns of A, 32 bytes of a row of B
-              const uint64_t desc = sw128_kmajor_desc(b + u * I::kUnit + (k >> 2) * (NT * 128) + (k & 3) * 32);
-              mma_tmem(tmem + kAccColumn + acc * NT, tmem + u * 64 + k * 8, desc, idesc, i > 0);
+              mma_tmem(d, from + k * 8, b + (((k >> 2) * (NT * 128) + (k & 3) * 32) >> 4), idesc, i > 0);
             }
             tc_commit(&d_full[acc]);
+            if (j == I::kGroups - 1) tc_commit(&a_empty[2 * per + u]);
+            if (j == I::kGroups - 1 && u == 1) tc_commit(&empty[st]);
           }
           __syncwarp();
           if (++acc == kAccs) acc = 0, acc_phase ^= 1;
         }
-        if (lane == 0 && ok) tc_commit(&a_empty[u]);
-        __syncwarp();
+        if (!ok) break;
       }
-      if (lane == 0 && ok) tc_commit(&empty[st]);
-      __syncwarp();
+      if (++st == kStages) st = 0, st_phase ^= 1;
+      if (++per == kPer) per = 0, per_phase ^= 1;
     }
   } else if (warp < 10) {
     const int u = (warp - 2) >> 2, quadrant = warp & 3, row = quadrant * 32 + lane;
-    const uint32_t to = tmem + ((uint32_t)(quadrant * 32) << 16) + u * 64;
+    const uint32_t lanes = tmem + ((uint32_t)(quadrant * 32) << 16);
+    int per = 0, per_phase = 1;
     for (int n = 0; n < end - begin && ok; ++n) {
       const int st = n % kStages;
       if (!(ok = wait(&full[st], (n / kStages) & 1))) break;
@@ -191,8 +197,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
       uint4 v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(w + ((4 * u + i) ^ (row & 7)) * 16);
-      if (n > 0 && !(ok = wait(&a_empty[u], (n - 1) & 1))) break;
+      if (!(ok = wait(&a_empty[2 * per + u], per_phase))) break;  // at once on its first round
       tc_fence_after();
+      const uint32_t to = lanes + (2 * per + u) * 64;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t r[32];
@@ -211,9 +218,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&a_full[u]);
+        mbar_arrive(&a_full[2 * per + u]);
         mbar_arrive(&empty[st]);
       }
+      if (++per == kPer) per = 0, per_phase ^= 1;
     }
   } else {
     const int half = (warp - 10) >> 2, quadrant = warp & 3, row = quadrant * 32 + lane;
