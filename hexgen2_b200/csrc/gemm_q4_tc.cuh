@@ -21,7 +21,7 @@ namespace tc {
 constexpr int kThreads = 18 * 32;
 constexpr int kRows = 128;
 constexpr int kWeightBytes = kRows * 128;  // of an item: 256 k
-constexpr int kAccs = 4;                   // accumulators in flight
+constexpr int kAccs = 2;                   // pairs of accumulators in flight
 
 // An item of a: two units of swizzled operands ([2 halves of 64 k][NT rows][128 bytes]), then (offset, factor)
 // [2 units][groups][NT].
@@ -33,8 +33,8 @@ struct Item {
   static constexpr int kBytes = 2 * kUnit + kStats;
   static constexpr int kPitch = (kWeightBytes + kBytes + 1023) / 1024 * 1024;  // of the ring
   static constexpr int kStages = NT == 64 ? 4 : NT == 32 ? 6 : 8;
-  // Operands of 64 columns in tensor memory, half of them for either unit; the accumulators behind them.
-  // (With one per unit its way round, unpack - MMA - free, took 3000 cycles an item.)
+  // Items whose operands (2 x 64 columns) are in tensor memory at a time; the accumulators behind them. (With
+  // one its way round, unpack - MMA - free, took 3000 cycles.)
   static constexpr int kPer = NT == 64 ? 2 : 3;
   static constexpr uint32_t kAccColumn = kPer * 2 * 64;
   static constexpr int kShared = kStages * kPitch + 1024;
@@ -113,12 +113,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
   constexpr uint32_t kAccColumn = I::kAccColumn;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  __shared__ uint64_t full[kStages], empty[kStages], a_full[2 * kPer], a_empty[2 * kPer], d_full[kAccs], d_empty[kAccs];
+  __shared__ uint64_t full[kStages], empty[kStages], a_full[kPer], a_empty[kPer], d_full[kAccs], d_empty[kAccs];
   __shared__ uint32_t tmem_at;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 17);
-    for (int i = 0; i < 2 * kPer; ++i) mbar_init(&a_full[i], 4), mbar_init(&a_empty[i], 1);
+    for (int i = 0; i < kPer; ++i) mbar_init(&a_full[i], 8), mbar_init(&a_empty[i], 1);
     for (int i = 0; i < kAccs; ++i) mbar_init(&d_full[i], 1), mbar_init(&d_empty[i], 8);
     fence_mbar_init();
   }
@@ -129,12 +129,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_at;
+  // All 512 columns begin at address 0. Known at compile time, the addresses of the MMAs stay in uniform
+  // registers; read back from shared memory they cost 80 cycles of moves per MMA.
+  constexpr uint32_t tmem = 0;
   pdl_wait();
   pdl_trigger();
   const Ranges ranges(total, gridDim.x);
   const int begin = ranges.begin(blockIdx.x), end = ranges.begin(blockIdx.x + 1);
-  bool ok = true;
+  bool ok = tmem_at == tmem;
+  if (!ok) record_device_error(HX_DEVERR_BAD_ARGUMENT);
 
   if (warp == 0) {
     int n = 0;
@@ -157,31 +160,30 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
     const uint64_t desc = sw128_kmajor_desc(smem_u32(smem + kWeightBytes));
     int acc = 0, acc_phase = 0, st = 0, st_phase = 0, per = 0, per_phase = 0;
     for (int n = 0; n < end - begin && ok; ++n) {
-      if (!(ok = wait(&full[st], st_phase))) break;
+      if (!(ok = wait(&full[st], st_phase) && wait(&a_full[per], per_phase))) break;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (!(ok = wait(&a_full[2 * per + u], per_phase))) break;
+      for (int j = 0; j < I::kGroups; ++j) {
+        if (!(ok = wait(&d_empty[acc], acc_phase ^ 1))) break;
         tc_fence_after();
+        if (lane == 0) {
+          const uint64_t b = desc + ((st * I::kPitch) >> 4);
+          const uint32_t d = tmem + kAccColumn + acc * 2 * NT, from = tmem + per * 128;
 #pragma unroll
-        for (int j = 0; j < I::kGroups; ++j) {
-          if (!(ok = wait(&d_empty[acc], acc_phase ^ 1))) break;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint64_t b = desc + ((st * I::kPitch + u * I::kUnit) >> 4);
-            const uint32_t d = tmem + kAccColumn + acc * NT, from = tmem + (2 * per + u) * 64;
+          for (int i = 0; i < G / 16; ++i)
 #pragma unroll
-            for (int i = 0; i < G / 16; ++i) {
+            for (int u = 0; u < 2; ++u) {
               const int k = j * (G / 16) + i;  // 16 k at a time: 8 columns of A, 32 bytes of a row of B
-              mma_tmem(d, from + k * 8, b + (((k >> 2) * (NT * 128) + (k & 3) * 32) >> 4), idesc, i > 0);
+              mma_tmem(d + u * NT, from + u * 64 + k * 8,
+                       b + ((u * I::kUnit + (k >> 2) * (NT * 128) + (k & 3) * 32) >> 4), idesc, i > 0);
             }
-            tc_commit(&d_full[acc]);
-            if (j == I::kGroups - 1) tc_commit(&a_empty[2 * per + u]);
-            if (j == I::kGroups - 1 && u == 1) tc_commit(&empty[st]);
+          tc_commit(&d_full[acc]);
+          if (j == I::kGroups - 1) {
+            tc_commit(&a_empty[per]);
+            tc_commit(&empty[st]);
           }
-          __syncwarp();
-          if (++acc == kAccs) acc = 0, acc_phase ^= 1;
         }
-        if (!ok) break;
+        __syncwarp();
+        if (++acc == kAccs) acc = 0, acc_phase ^= 1;
       }
       if (++st == kStages) st = 0, st_phase ^= 1;
       if (++per == kPer) per = 0, per_phase ^= 1;
@@ -197,9 +199,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
       uint4 v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4*>(w + ((4 * u + i) ^ (row & 7)) * 16);
-      if (!(ok = wait(&a_empty[2 * per + u], per_phase))) break;  // at once on its first round
+      if (!(ok = wait(&a_empty[per], per_phase))) break;  // at once on its first round
       tc_fence_after();
-      const uint32_t to = lanes + (2 * per + u) * 64;
+      const uint32_t to = lanes + per * 128 + u * 64;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t r[32];
@@ -218,7 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&a_full[2 * per + u]);
+        mbar_arrive(&a_full[per]);
         mbar_arrive(&empty[st]);
       }
       if (++per == kPer) per = 0, per_phase ^= 1;
@@ -249,22 +251,28 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
       if (!(ok = wait(&full[st], (n / kStages) & 1))) break;
       const uint8_t* stats = smem + st * I::kPitch + kWeightBytes + 2 * I::kUnit + half * kHalf * 8;
 #pragma unroll
-      for (int i = 0; i < 2 * I::kGroups; ++i) {
+      for (int j = 0; j < I::kGroups; ++j) {
         if (!(ok = wait(&d_full[acc], acc_phase))) break;
         tc_fence_after();
-        uint32_t d[kHalf];
-        tmem_ld(from + acc * NT, d);
-        tc_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&d_empty[acc]);
-        if (++acc == kAccs) acc = 0, acc_phase ^= 1;
 #pragma unroll
-        for (int m = 0; m < kHalf; m += 2) {
-          const float4 f = *reinterpret_cast<const float4*>(stats + (i * NT + m) * 8);
-          tot[m] = fmaf(s[i], fmaf(__uint_as_float(d[m]), f.y, f.x), tot[m]);
-          tot[m + 1] = fmaf(s[i], fmaf(__uint_as_float(d[m + 1]), f.w, f.z), tot[m + 1]);
+        for (int u = 0; u < 2; ++u) {
+          const int i = u * I::kGroups + j;
+          uint32_t d[kHalf];
+          tmem_ld(from + (acc * 2 + u) * NT, d);
+          tc_wait_ld();
+          if (u == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&d_empty[acc]);
+          }
+#pragma unroll
+          for (int m = 0; m < kHalf; m += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(stats + (i * NT + m) * 8);
+            tot[m] = fmaf(s[i], fmaf(__uint_as_float(d[m]), f.y, f.x), tot[m]);
+            tot[m + 1] = fmaf(s[i], fmaf(__uint_as_float(d[m + 1]), f.w, f.z), tot[m + 1]);
+          }
         }
+        if (++acc == kAccs) acc = 0, acc_phase ^= 1;
       }
       if (!ok) break;
       __syncwarp();
@@ -289,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem_at, 512);
   }
 }
 
