@@ -99,9 +99,6 @@ __global__ void __launch_bounds__(kThreads) gemm_q4_kernel(const Args p) {
 //   third of the instructions. Weights by plain loads, eight rows to an instruction, kept L1's tags 75 %
 //   busy at a quarter of the memory's bandwidth; bulk copies of 128 bytes took about 20 cycles each.
 // ------------------------------------------------------------------------------------------
-#ifndef HX_TC_MIN
-#define HX_TC_MIN 0
-#endif
 constexpr int kWarps = 16;
 constexpr int kMmaThreads = kWarps * 32;
 constexpr int kUnitK = 128;
@@ -448,8 +445,11 @@ Plan plan(int64_t m, int64_t n, int64_t k, bool gated) {
   return pl;
 }
 
-// Whether the tcgen05 kernel takes a product.
-bool use_tc(int64_t m, int64_t n, int64_t k) { return m > 8 && n * k >= HX_TC_MIN; }
+// Whether the tcgen05 kernel takes a product: its three launches cost about 8 us whatever the size, its items
+// less than the passes that 17 and more rows take here. Measured, us here / there (bf16, groups of 128,
+// m x n x k): 24x4096x4096 15.3 / 15.8, 64x4096x4096 20.8 / 18.4, 32x22016x4096 42.6 / 32.4,
+// 64x22016x4096 69 / 38.5, 64x1024x1024 6.0 / 9.6; in one pass 16x12288x4096 20.4 / 22.0.
+bool use_tc(int64_t m, int64_t n, int64_t k) { return m > 16 && m * n * k >= int64_t(1) << 29; }
 
 template <typename T, int G, int NT, int EPI>
 int launch_mma(const Args& p, float* running, cudaStream_t stream) {

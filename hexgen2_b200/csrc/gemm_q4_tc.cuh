@@ -1,4 +1,4 @@
-// gemm_q4 on tcgen05: large weights times 9 to 64 rows of a (gemm_q4.cu has the operator and its other kernels).
+// gemm_q4 on tcgen05: large weights times 17 to 64 rows of a (gemm_q4.cu has the operator and its other kernels).
 //
 // D[128 weight rows, NT rows of a] = A B^T by tcgen05.mma kind::f16, M = 128. A, the codes, is made in tensor
 // memory: the bits of a code are an f16 as they stand (codes * 2^-24, or 2^-20 one nibble up), so a
@@ -14,6 +14,11 @@
 //   10-17  accumulate: tensor memory -> registers, four warps (a lane per weight row) for either half of
 //          a's rows; at the end of a block's part they write it to the workspace
 // join_kernel adds the parts of a block up in CTA order and applies the epilogue.
+//
+// What bounds it: the issue of the MMAs. 32 x 22016 x 4096 (SwiGLU, groups of 128) takes 32 us for 7.3 us of
+// bytes: 8 us for the three launches, then 18.6 items of 2300 cycles per SM, of which the one thread
+// that issues spends 1000 on its 16 MMAs (62 cycles each at 32 rows, the tensor pipe needs 16), 250 on
+// commits and the rest waiting.
 #pragma once
 
 namespace tc {
@@ -32,7 +37,7 @@ struct Item {
   static constexpr int kStats = 2 * kGroups * NT * 8;
   static constexpr int kBytes = 2 * kUnit + kStats;
   static constexpr int kPitch = (kWeightBytes + kBytes + 1023) / 1024 * 1024;  // of the ring
-  static constexpr int kStages = NT == 64 ? 4 : NT == 32 ? 6 : 8;
+  static constexpr int kStages = NT == 64 ? 4 : 6;
   // Items whose operands (2 x 64 columns) are in tensor memory at a time; the accumulators behind them. (With
   // one its way round, unpack - MMA - free, took 3000 cycles.)
   static constexpr int kPer = NT == 64 ? 2 : 3;
@@ -98,11 +103,6 @@ HX_DEVICE void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint
 }
 HX_DEVICE void tmem_ld(uint32_t addr, uint32_t (&r)[32]) { tmem_ld_32x32b_x32(addr, r); }
 HX_DEVICE void tmem_ld(uint32_t addr, uint32_t (&r)[16]) { tmem_ld_32x32b_x16(addr, r); }
-HX_DEVICE void tmem_ld(uint32_t addr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(addr));
-}
 
 template <typename T, int G, int NT>
 __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
@@ -289,9 +289,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_q4_tc_kernel(
       else ++item;
     }
   }
-  if (!ok && warp == 1) {  // whatever was issued ends before tensor memory goes
-    if (lane == 0) tc_commit(&a_empty[0]);
-    __nanosleep(1000000);
+  if (!ok && warp == 1) {  // whatever was issued ends before tensor memory goes: a commit behind it, waited for
+    __shared__ uint64_t drained;
+    if (lane == 0) {
+      mbar_init(&drained, 1);
+      fence_mbar_init();
+      tc_commit(&drained);
+      mbar_wait_drain(&drained, 0);
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -331,7 +337,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Args p, const float* __
 }
 
 inline int items(int64_t k) { return ceil_div(k, 256); }
-inline int rows_of_a(int64_t m) { return m <= 16 ? 16 : m <= 32 ? 32 : 64; }
+inline int rows_of_a(int64_t m) { return m <= 32 ? 32 : 64; }
 
 // Workspace: the staged rows of a, then the parts.
 inline size_t staged_bytes(int64_t m, int64_t k, int64_t group) {
@@ -373,9 +379,7 @@ int launch(const Args& p, int epilogue, void* ws, cudaStream_t stream) {
 
 template <typename T, int G>
 int launch_rows(const Args& p, int epilogue, void* ws, cudaStream_t stream) {
-  return p.M <= 16   ? launch<T, G, 16>(p, epilogue, ws, stream)
-         : p.M <= 32 ? launch<T, G, 32>(p, epilogue, ws, stream)
-                     : launch<T, G, 64>(p, epilogue, ws, stream);
+  return p.M <= 32 ? launch<T, G, 32>(p, epilogue, ws, stream) : launch<T, G, 64>(p, epilogue, ws, stream);
 }
 
 }  // namespace tc

@@ -493,7 +493,7 @@ def gemm_q4(a, w_q4, scales, epilogue=HX_EPI_NONE, residual=None, out=None):
           K, group, a.stride(0) if M > 1 else max(K, a.stride(0)),
           out.stride(0) if M > 1 else cols, epilogue, _p(residual),
           0 if residual is None else residual.stride(0) if M > 1 else cols, _p(ws), nbytes, code)
-    _count(1)
+    _count(3 if M > 16 and nbytes else 1)
     return out
 
 

@@ -410,7 +410,10 @@ def linear64(a, codes, scales, epilogue, residual):
     (1, 1, 32, 32, 0), (1, 7, 96, 32, 1), (2, 33, 128, 128, 0), (3, 64, 192, 64, 2), (1, 4096, 1024, 128, 1),
     (8, 100, 512, 128, 1), (9, 160, 640, 64, 2), (16, 257, 4096, 128, 0), (17, 96, 2208, 32, 2),
     (31, 130, 1152, 128, 1), (33, 64, 256, 64, 2), (64, 515, 1088, 64, 0), (64, 1024, 2048, 128, 1),
-    (3, 96, 8320, 64, 2), (8, 50, 16512, 128, 1), (20, 64, 4128, 32, 2), (40, 40, 8448, 128, 0)])
+    (3, 96, 8320, 64, 2), (8, 50, 16512, 128, 1), (20, 64, 4128, 32, 2), (40, 40, 8448, 128, 0),
+    # large enough for the tcgen05 kernel
+    (17, 8005, 4096, 128, 1), (32, 4128, 4160, 64, 2), (33, 4000, 4224, 64, 0), (64, 2080, 4128, 32, 2),
+    (50, 1100, 11008, 128, 1)])
 def test_gemm_q4(dtype, M, N, K, group, epilogue):
     dt = DT[dtype]
     g = torch.Generator().manual_seed(M * N + K)
