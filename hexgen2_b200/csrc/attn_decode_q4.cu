@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
   int done = 0;
   for (; done < n_tiles; ++done) {
     const int stage = done % kStages;
-    if (!mbar_wait_warp(&full[warp][stage], (done / kStages) & 1)) break;
+    if (!mbar_wait_warp_timed(&full[warp][stage], (done / kStages) & 1)) break;
     const uint8_t* tile = ring + stage * (kTile * kRec);
     const int n = end - (first + done * (kWarps * kTile));
     if (n >= kTile)

@@ -165,6 +165,21 @@ HX_DEVICE bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 
+// mbar_wait_warp for kernels whose other outputs stay good when some call has set the error word (a bad
+// length cut and reported, say): only time ends this wait.
+HX_DEVICE bool mbar_wait_warp_timed(uint64_t* bar, uint32_t parity) {
+  bool done = mbar_try_wait(bar, parity);
+  if (!done) {
+    const unsigned long long t0 = globaltimer_ns();
+    do {
+#pragma unroll 1
+      for (int i = 0; i < 64 && !done; ++i) done = mbar_try_wait(bar, parity);
+    } while (!done && globaltimer_ns() - t0 <= HX_WAIT_LIMIT_NS);
+    if (!done) record_device_error(HX_DEVERR_WAIT_TIMEOUT);
+  }
+  return __all_sync(0xffffffffu, done);
+}
+
 // AND-reduction of a predicate over the `count` threads of named barrier `id` (warp-aligned).
 // Lets a group of warps take a common decision (e.g. all abort after a timed-out wait) so that
 // no warp is left waiting at a later named barrier.

@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) gemm_q4_mma_kernel(
           for (int q = 0; q < kScales; ++q) s[h][q] = DT<T>::to_f(next[h][q]) * 1048576.f;
         if (pair + 1 < mine) ask_scales(step, pair + 1);
         else if (step + 1 < steps) ask_scales(step + 1, 0);
-        if (ok) ok = mbar_wait_warp(&full[warp][st], phase);
+        if (ok) ok = mbar_wait_warp_timed(&full[warp][st], phase);
         if (!ok) break;
         multiply<T, G, NT>(ring + st * kStageBytes, s, sm_a + (kw + (pair << pl.log_kw)) * (kPair * B::kBytes), tot);
         __syncwarp();

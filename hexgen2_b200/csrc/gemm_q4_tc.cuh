@@ -78,19 +78,7 @@ __global__ void __launch_bounds__(256) stage_kernel(const Args p, uint8_t* __res
   }
 }
 
-// Bounded wait of a whole warp, by time alone (an error some other call has left must not end it).
-HX_DEVICE bool wait(uint64_t* bar, uint32_t parity) {
-  bool done = mbar_try_wait(bar, parity);
-  if (!done) {
-    const unsigned long long t0 = globaltimer_ns();
-    do {  // the timer is far away: a look at it costs as much as a product of a unit
-#pragma unroll 1
-      for (int i = 0; i < 256 && !done; ++i) done = mbar_try_wait(bar, parity);
-    } while (!done && globaltimer_ns() - t0 <= HX_WAIT_LIMIT_NS);
-    if (!done) record_device_error(HX_DEVERR_WAIT_TIMEOUT);
-  }
-  return __all_sync(0xffffffffu, done);
-}
+HX_DEVICE bool wait(uint64_t* bar, uint32_t parity) { return mbar_wait_warp_timed(bar, parity); }
 
 // D(tmem) (+)= A(tmem) * B(smem desc)^T, f16 operands, f32 sums.
 HX_DEVICE void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {

@@ -490,7 +490,7 @@ def gemm_q4(a, w_q4, scales, epilogue=HX_EPI_NONE, residual=None, out=None):
         nbytes = _L().hx_gemm_q4_workspace(M, N, K, group, code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=a.device) if nbytes else None
     _call(dev, _L().hx_gemm_q4, a.data_ptr(), w_q4.data_ptr(), scales.data_ptr(), out.data_ptr(), M, N,
-          K, group, a.stride(0) if M > 1 else max(K, a.stride(0)),
+          K, group, a.stride(0) if M > 1 else K,
           out.stride(0) if M > 1 else cols, epilogue, _p(residual),
           0 if residual is None else residual.stride(0) if M > 1 else cols, _p(ws), nbytes, code)
     _count(3 if M > 16 and nbytes else 1)

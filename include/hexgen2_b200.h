@@ -281,7 +281,8 @@ size_t hx_decode_attention_q4_workspace(int64_t batch, int64_t n_heads, int64_t 
  * contiguous (element 2j in the low nibble of byte j), scales: [n, k/group] contiguous in dtype,
  * group 32, 64 or 128 dividing k. Epilogues NONE, RESIDUAL (+ residual[m, n]) and SWIGLU (rows of
  * w interleaved [up16|gate16], c has n/2 columns), as hx_gemm's but in f32 up to the one rounding.
- * a 16-byte aligned with lda a multiple of 16 bytes; w 16-byte aligned. residual may be c.
+ * A row of a with an infinity or NaN gives NaN (f16/bf16). a 16-byte aligned with lda a multiple of
+ * 16 bytes; w 16-byte aligned. residual may be c.
  * workspace: hx_gemm_q4_workspace() bytes (f16/bf16: running sums where k is above 8192, or 4096
  * with more than eight rows; staged rows and partial sums of large products of more than 16 rows), not
  * shared by calls that may overlap. No counterpart in the reference. */

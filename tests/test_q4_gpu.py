@@ -468,6 +468,33 @@ def test_gemm_q4_rows_do_not_mix():
     assert out[11].isnan().all()
 
 
+def test_one_row_of_any_stride():
+    """A single row of a whose stride is not a multiple of 16 bytes."""
+    g = torch.Generator().manual_seed(2)
+    codes, scales = (t.cuda() for t in quantize_weight_q4(torch.randn(48, 64, generator=g).bfloat16(), 32))
+    row = torch.randn(1, 67, generator=g).bfloat16().cuda()[:, :64]
+    assert torch.equal(ops.gemm_q4(row, codes, scales), ops.gemm_q4(row.contiguous(), codes, scales))
+
+
+def test_an_error_left_by_another_call_spoils_nothing():
+    """The device error word is set (a count beyond the cache) and not yet read: products and
+    attention still wait for their data."""
+    g = torch.Generator().manual_seed(8)
+    codes, scales = (t.cuda() for t in quantize_weight_q4(torch.randn(4096, 4096, generator=g).bfloat16(), 128))
+    xs = [torch.randn(m, 4096, generator=g).bfloat16().cuda() for m in (1, 12, 40)]
+    rec = make_cache(2, 4, 3000, 128, g, torch.bfloat16, 0.3).cuda()
+    q = torch.randn(2, 4, 128, generator=g).bfloat16().cuda()
+    lens = i32([3000, 1500])
+    run = lambda: [ops.gemm_q4(x, codes, scales) for x in xs] + [ops.decode_attention_q4(q, rec, lens, 4, 3000, 0.1)]  # noqa: E731
+    clean = run()
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    ops.quantize_cache_q4(torch.zeros(1, 2, 2, 1, 32, device="cuda"), i32([3]), ops.allocate_cache_q4(1, 1, 2, 32))
+    for _ in range(3):
+        flush.zero_()  # weights and records come from HBM again
+        assert all(torch.equal(a, b) for a, b in zip(run(), clean))
+    assert ops.device_error() == 2
+
+
 # ------------------------------------------------------------------------------ together
 def layer(x, res, w, cos, sin, q4, pos, seqlens, hq, hk, d, cap, head):
     """One decode step of one layer and the LM head, in 4 bits."""
