@@ -85,6 +85,15 @@ HX_DEVICE Key peek(const Key* p, int rank, int C) {
 // |d| 2^-24 of itself.
 HX_DEVICE float exp_neg(float d) { return ex2_approx(d * 1.4426950408889634f); }
 
+// z = sum exp(x - m) and s = sum exp(x - m) (x - m) move to a larger maximum, d = m - maximum <= 0. Logits
+// masked with a type's lowest value make d as low as -3.4e38, and d z would overflow; below -1000 exp(d) is 0
+// already, so d stops there. A NaN (from infinities) stays in z.
+HX_DEVICE void rebase(float d, float& z, float& s) {
+  const float f = exp_neg(d);
+  s = fmaf(fmaxf(d, -1000.f), z, s) * f;
+  z *= f;
+}
+
 // row[begin, end) as thread `tid` of kThreads sees it: an element up to a 16-byte boundary, vectors tid, tid +
 // kThreads, ... of 16 bytes, an element behind them.
 template <typename T>
@@ -192,11 +201,7 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(
     }
     if (where < 0) where = at, width = V;
     if (top > m) {
-      if (m != -INFINITY) {
-        const float d = m - top, f = exp_neg(d);
-        s = fmaf(d, z, s) * f;
-        z *= f;
-      }
+      if (m != -INFINITY) rebase(m - top, z, s);
       m = top;
       int at_u = 0;
 #pragma unroll
@@ -223,11 +228,7 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(
   top = sm_max[0];
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) top = fmaxf(top, sm_max[w]);
-  if (m != -INFINITY) {
-    const float d = m - top, f = exp_neg(d);
-    s = fmaf(d, z, s) * f;
-    z *= f;
-  }
+  if (m != -INFINITY) rebase(m - top, z, s);
   z = warp_sum(z);
   s = warp_sum(s);
   if (lane == 0) sm_z[warp] = z, sm_s[warp] = s;
@@ -263,11 +264,11 @@ __global__ void __launch_bounds__(kThreads, 8) logprobs_kernel(
   {
     const bool some = lane < C;
     const float mc = some ? peek(&sm_total[0], lane, C) : -INFINITY;
-    const float zc = some ? peek(&sm_total[1], lane, C) : 0.f, sc = some ? peek(&sm_total[2], lane, C) : 0.f;
+    float zc = some ? peek(&sm_total[1], lane, C) : 0.f, sc = some ? peek(&sm_total[2], lane, C) : 0.f;
     top = warp_max(mc);
-    const float d = mc - top, f = mc == -INFINITY ? 1.f : exp_neg(d);  // without a maximum: 0, or NaN to keep
-    z = warp_sum(zc * f);
-    s = warp_sum((mc == -INFINITY ? sc : fmaf(d, zc, sc)) * f);
+    if (mc != -INFINITY) rebase(mc - top, zc, sc);  // without a maximum: 0, or NaN to keep
+    z = warp_sum(zc);
+    s = warp_sum(sc);
   }
   if (top == -INFINITY) z = NAN;
   const float log_z = logf(z);

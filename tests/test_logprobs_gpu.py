@@ -126,3 +126,34 @@ def test_flat_peaked_and_far_rows(scale, offset):
     x = scale * torch.randn(3, 9000, generator=g) + offset
     tokens = torch.tensor([0, 4500, 8999])
     check(x, tokens, 5, ops.token_logprobs(x.cuda(), tokens.cuda(), top_k=5, entropy=True))
+
+
+MASKS = {  # which logits of a row of v are masked
+    "leading half": lambda i, v: i < v // 2,  # whole slices of a cluster
+    "all but three": lambda i, v: i < v - 3,
+    "all but one in front": lambda i, v: i > 0,
+    "every other run of 64": lambda i, v: i // 64 % 2 == 0,
+    "half of the threads": lambda i, v: i // 8 % 128 < 64,  # by 16-byte vectors of 16-bit logits
+    "one in seven left": lambda i, v: i % 7 != 0,
+}
+
+
+@pytest.mark.parametrize("dtype,mask", [("f32", -1000.0), ("f32", -1e9), ("f32", -1e35), ("f32", -1e38), ("f32", "min"),
+                                        ("bf16", -1e35), ("bf16", "min"), ("f16", "min")])
+@pytest.mark.parametrize("rows,vocab", [(6, 40), (6, 777), (6, 4096), (12, 33001), (1302, 2100)])
+def test_logits_masked_with_low_finite_values(dtype, mask, rows, vocab):
+    """Masked logits of the type's lowest value, or any other low one, leave finite sums: each pattern in its own
+    rows, and rows of masked logits alone (equal logits: the entropy is log vocab)."""
+    dt = DT[dtype]
+    low = torch.finfo(dt).min if mask == "min" else mask
+    g = torch.Generator().manual_seed(rows + vocab)
+    x = torch.randn(rows + 1, vocab, generator=g)
+    i = torch.arange(vocab)
+    for r, pattern in zip(range(rows), list(MASKS.values()) * rows):
+        x[r, pattern(i, vocab)] = low
+    x[rows] = low
+    x = x.to(dt)
+    tokens = torch.randint(0, vocab, (rows + 1,), generator=g)
+    got = ops.token_logprobs(x.cuda(), tokens.cuda(), top_k=5, entropy=True)
+    assert got.entropy.isfinite().all() and got.logprobs.isfinite().all()
+    check(x, tokens, 5, got)
