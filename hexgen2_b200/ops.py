@@ -407,7 +407,8 @@ def rotary_cache_write_q4(qkv, batch, seqlen, n_heads, n_heads_kv, head_dim, pos
     if qkv.numel() != batch * seqlen * (n_heads + 2 * n_heads_kv) * head_dim or not qkv.is_contiguous():
         raise ValueError(f"{what}: qkv must be contiguous [batch, seqlen, (n_heads + 2 n_heads_kv) * head_dim]")
     for t in (cos, sin):
-        if t.dtype != qkv.dtype or t.shape != cos.shape or t.shape[-1] * 2 != head_dim or not t.is_contiguous():
+        if (t.dim() != 2 or t.dtype != qkv.dtype or t.shape != cos.shape or t.shape[1] * 2 != head_dim
+                or not t.is_contiguous()):
             raise ValueError(f"{what}: cos and sin must be contiguous [positions, head_dim / 2] in qkv's dtype")
     dev = _device_of(qkv, cache_q4, pos_start, cos, sin, q_out)
     if q_out is None:

@@ -98,6 +98,17 @@ def test_bad_arguments_are_refused(call, match):
         call(torch.zeros(2, 8, 2, 2, 32))
 
 
+@pytest.mark.parametrize("shape", [(16,), (1, 16), (1, 8, 16), (8, 1, 16), (8, 2, 8)])
+def test_rotary_tables_have_a_row_for_each_position(shape):
+    """Tables of another rank are refused: the kernel takes the first size for the number of rows (16 rows of 16 in a
+    table of 16 values would be read past its end). One row is a table of one position."""
+    def call():
+        t = torch.zeros(shape)
+        ops.rotary_cache_write_q4(torch.zeros(2, 6 * 32), 2, 1, 2, 2, 32, i32(0, 0), t, t, q4())
+    with pytest.raises(ValueError, match="CUDA" if shape == (1, 16) else "cos and sin"):
+        call()
+
+
 P = 1 << 20  # an aligned address that is never followed: every call below fails its checks first
 
 
