@@ -180,8 +180,11 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
 //     the words it can read with one wide load: for S 1/4 of a position's K codes, for O 1/8 of
 //     a position's V codes (bytes of two positions joined with one permute).
 //   - P' enters as f16, relative to the largest P' seen (the running reference r follows
-//     s + log2 v_scale, not s): 2^-12 of each value, 2^-25 * 2^-7 of the largest. For f16 outputs, whose
-//     half step is no coarser than that, P' is the sum of two f16.
+//     s + log2 v_scale, not s): at most 2^-11 of each value off, and 2^-25 * 2^-7 of the largest. So that this
+//     moves a value's distance from the middle of its row and not its codes, which are many times the output
+//     where values average out, the codes are taken about 7.5: the rounded P' times 7.5 go off again in f32, the
+//     middle v_min + 7.5 v_scale comes in with p itself. For f16 outputs, whose half step is no coarser, P' is
+//     the sum of two f16 (2^-22).
 //   - S comes out position-major; movmatrix turns it into the B operand of O.
 // Each warp streams 32-position tiles through a ring of its own (bulk copies by its lane 0, one
 // mbarrier per stage): no block barrier until the warps' partials are added up at the end.
@@ -235,8 +238,9 @@ struct McSmem {
 };
 
 // State of one warp's online softmax. Per lane, for columns 2t + j of each tile of eight: the
-// reference r (the same in all lanes of equal t), this lane's shares of sum p and sum p v_min, and
-// the output elements of its rows, even elements times 2^-24, odd ones times 2^-20.
+// reference r (the same in all lanes of equal t), this lane's shares of sum p and of what all output elements
+// have in common (z: sum p v_min, or p times the rows' middles less 7.5 sum P'), and the output elements of
+// its rows, even elements times 2^-24, odd ones times 2^-20.
 template <int D, int NT, int NJ>
 struct Softmax {
   float r[NT][NJ], l[NT][NJ], z[NT][NJ], o[NT][D / 16][4];
@@ -343,21 +347,25 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const bool live = kFull || sub * 16 + r * 8 + g < n;  // stale scales may be NaN
+        const float base = kTwo ? meta[sub][r].w : fmaf(7.5f, meta[sub][r].z, meta[sub][r].w);
         float pv[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           const float p = ex2_approx(s[sub][nt][2 * r + j] - st.r[nt][j]);
           if (live) {
             st.l[nt][j] += p;
-            st.z[nt][j] = fmaf(p, meta[sub][r].w, st.z[nt][j]);
+            st.z[nt][j] = fmaf(p, base, st.z[nt][j]);
             pv[j] = p * meta[sub][r].z;
           }
         }
         const uint32_t hi = pack2<__half>(pv[0], pv[1]);
         bh[nt][r] = transpose8x8(hi);
-        if (kTwo) {
-          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        if constexpr (kTwo) {
           bl[nt][r] = transpose8x8(pack2<__half>(pv[0] - back.x, pv[1] - back.y));
+        } else {
+          st.z[nt][0] = fmaf(-7.5f, back.x, st.z[nt][0]);
+          if constexpr (NJ == 2) st.z[nt][1] = fmaf(-7.5f, back.y, st.z[nt][1]);
         }
       }
     // V codes of positions 2t, 2t + 1, 2t + 8, 2t + 9: lane (g, t) takes bytes [D/16 g, D/16 (g + 1)).
