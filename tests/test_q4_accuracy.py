@@ -73,8 +73,8 @@ def test_the_bound_bites(hq, hk, d, lens, scale):
     dt = torch.bfloat16
     for wide in (False, True):
         q, rec, keep = case(hq, hk, d, lens, wide, dt)
-        want, bound = attention64(q, rec, lens, scale, 8, keep)
-        is_far = lambda **kw: far(emulated(q, rec, lens, scale, dt, 512, **kw)[..., keep], want, bound, dt)  # noqa: E731
+        want, bound = attention64(q, rec, lens, scale, splits_of(len(lens), hq, hk, d, max(lens)), keep)
+        is_far = lambda **kw: far(emulated(q, rec, lens, scale, dt, 128, **kw)[..., keep], want, bound, dt)  # noqa: E731
         assert is_far() <= 1
         assert far(torch.zeros_like(want), want, bound, dt) > 50
         assert is_far(lose=1) > 1 and is_far(merge=False) > 1
