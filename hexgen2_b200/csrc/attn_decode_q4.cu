@@ -180,11 +180,11 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
 //     the words it can read with one wide load: for S 1/4 of a position's K codes, for O 1/8 of
 //     a position's V codes (bytes of two positions joined with one permute).
 //   - P' enters as f16, relative to the largest P' seen (the running reference r follows
-//     s + log2 v_scale, not s): at most 2^-11 of each value off, and 2^-25 * 2^-7 of the largest. So that this
-//     moves a value's distance from the middle of its row and not its codes, which are many times the output
-//     where values average out, the codes are taken about 7.5: the rounded P' times 7.5 go off again in f32, the
-//     middle v_min + 7.5 v_scale comes in with p itself. For f16 outputs, whose half step is no coarser, P' is
-//     the sum of two f16 (2^-22).
+//     s + log2 v_scale, not s, down to v_scale = 2^-80): at most 2^-11 of each value off, and
+//     2^-25 * 2^-7 of the largest. So that this moves a value's distance from the middle of its row and not
+//     its codes, which are many times the output where values average out, the codes are taken about 7.5:
+//     the rounded P' times 7.5 go off again in f32, the middle v_min + 7.5 v_scale comes in with p itself.
+//     For f16 outputs, whose half step is no coarser, P' is the sum of two f16 (2^-22).
 //   - S comes out position-major; movmatrix turns it into the B operand of O.
 // Each warp streams 32-position tiles through a ring of its own (bulk copies by its lane 0, one
 // mbarrier per stage): no block barrier until the warps' partials are added up at the end.
@@ -246,7 +246,14 @@ struct Softmax {
   float r[NT][NJ], l[NT][NJ], z[NT][NJ], o[NT][D / 16][4];
 };
 
-constexpr float kFloor = -32.f;  // log2 of the smallest v_scale that the reference follows
+// What the reference follows of a row's values is log2 of v_scale, or of 2^-24 |v_min| where that is more (flat rows,
+// so that p v_min stays finite), but no less than this (rows of zeros): p then stays below 2^95, a sum of 2^30
+// of them in f32, and a P' of the smallest v_scale that records have (2^-104) is still 2^-17 or more at the top.
+constexpr float kFloor = -80.f;
+
+// Sums move to a reference that is 2^(2 log2 half) higher. A row of zeros may be 2^200 away from one of large values:
+// the factor is 0 in f32 then, as it may be for o and z, but not for l.
+HX_DEVICE float scale_l(float l, float half) { return l * half * half; }
 
 // One tile of n positions (kFull: n = kTile) in shared memory.
 template <typename T, int D, int NT, int NJ, bool kFull>
@@ -302,7 +309,7 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float ks = meta[sub][r].x * scale_log2, km = meta[sub][r].y * scale_log2;
-      const float lv = fmaxf(lg2_approx(meta[sub][r].z), kFloor);
+      const float lv = fmaxf(lg2_approx(fmaxf(meta[sub][r].z, fabsf(meta[sub][r].w) * 0x1p-24f)), kFloor);
       const bool live = kFull || sub * 16 + r * 8 + g < n;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -331,9 +338,10 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const float next = fmaxf(st.r[nt][j], top[nt][j] - 7.f);
-        const float f = ex2_approx(st.r[nt][j] - next);
+        const float half = ex2_approx(0.5f * (st.r[nt][j] - next));
         st.r[nt][j] = next;
-        st.l[nt][j] *= f;
+        const float f = half * half;
+        st.l[nt][j] = scale_l(st.l[nt][j], half);
         st.z[nt][j] *= f;
 #pragma unroll
         for (int i = 0; i < OT; ++i) st.o[nt][i][j] *= f, st.o[nt][i][2 + j] *= f;
@@ -552,9 +560,9 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       if (start + w * kTile >= end) continue;  // this warp had no positions
-      const float f = exp2f(sm_m[w][q] - M);
-      L += f * sm_l[w][q];
-      O += f * sm_o[w * kHeads * D + i];
+      const float half = exp2f(0.5f * (sm_m[w][q] - M));
+      L += scale_l(sm_l[w][q], half);
+      O += half * half * sm_o[w * kHeads * D + i];
     }
     if (a.splits == 1) {
       out[i] = DT<T>::from_f(O / L);
@@ -580,9 +588,9 @@ __global__ void __launch_bounds__(D) decode_q4_merge_kernel(const Args a) {
   float M = -INFINITY, L = 0.f, O = 0.f;
   for (int s = 0; s < n; ++s) M = fmaxf(M, ml[2 * s]);
   for (int s = 0; s < n; ++s) {
-    const float f = exp2f(ml[2 * s] - M);
-    L += f * ml[2 * s + 1];
-    O += f * o[(int64_t)s * D];
+    const float half = exp2f(0.5f * (ml[2 * s] - M));
+    L += scale_l(ml[2 * s + 1], half);
+    O += half * half * o[(int64_t)s * D];
   }
   ((T*)a.out)[bh * D + threadIdx.x] = DT<T>::from_f(n ? O / L : 0.f);
 }

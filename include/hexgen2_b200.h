@@ -264,7 +264,8 @@ int hx_rotary_cache_write_q4(const void* qkv, int64_t batch, int64_t seqlen, int
  * q_batch_stride elements), sequence b attends to the first seqlens_k[b] records of each KV head
  * of cache_q4[b]; out [batch, n_heads, head_dim] contiguous. Any number of query heads per KV
  * head. A sequence of length 0 gives zeros; a length above max_seqlen_k (or below 0) is cut to it
- * and sets the device error word to 2. workspace: hx_decode_attention_q4_workspace() bytes, not
+ * and sets the device error word to 2. f16/bf16: queries and values up to 2^100 in size, full digits of
+ * values whose scale is 2^-80 or more. workspace: hx_decode_attention_q4_workspace() bytes, not
  * shared by calls that may overlap. */
 int hx_decode_attention_q4(const void* q, int64_t q_batch_stride, const void* cache_q4,
                            int64_t q4_batch_stride, int64_t q4_head_stride,

@@ -31,12 +31,12 @@ def parts64(rec):
     return c[..., :d], meta[..., :1], meta[..., 1:2], c[..., d:], meta[..., 2:3], meta[..., 3:]
 
 
-def attention64(q, rec, lens, scale, splits, keep=slice(None)):
+def attention64(q, rec, lens, scale, splits, keep=slice(None), least=2.0 ** -32):
     """Attention of q [B, hq, d] over the first lens[b] records of rec [B, hkv, S, d + 16] in 64 bits, and a bound
     [B, hq] on the 2-norm, over the outputs `keep`, of the error of f32 sums in up to `splits` parts, before the output
     rounds to its type. All outputs that are not in `keep` are left out. With w the softmax weights, c a position's codes, vs and mid = vmin + 7.5 vs its scale and middle:
       - weights times vs enter as f16, each off by at most half a step, 2^-11, at random (so 2^-11 / sqrt(3) rms), and by
-        2^-32 of the largest. As mid is added apart, that moves vs (c - 7.5): twice the rms of the sum's norm.
+        `least` of the largest. As mid is added apart, that moves vs (c - 7.5): twice the rms of the sum's norm.
         (f16 outputs take two f16 a weight, 2^-22; the bound is that of one all the same.)
       - a score is off by delta = scale sum|q| (15 ks (d / 16 + 3) + 2 |kmin|) 2^-23 (a sum of d / 16 matrix products,
         the sum of q, scaling) and 2^-22 |s| (the product's rounding at the exponential's), and the exponential by
@@ -60,7 +60,7 @@ def attention64(q, rec, lens, scale, splits, keep=slice(None)):
             out[b, h] = o
             off = vs * (vc - 7.5)
             rounding = 2 * 2.0 ** -11 / 3 ** 0.5 * (w * off).square().sum().sqrt()
-            rounding = rounding + n * 2.0 ** -32 * (w * vs).max() * 7.5 * vc.shape[1] ** 0.5
+            rounding = rounding + n * least * (w * vs).max() * 7.5 * vc.shape[1] ** 0.5
             delta = scale * x.abs().sum() * (15 * ks * (d / 16 + 3) + 2 * km.abs()) * 2.0 ** -23
             delta = delta + (s[:, None].abs() + 2) * 2.0 ** -22
             scores = (w * delta * (v - o).abs()).sum(0).norm()

@@ -43,6 +43,38 @@ def test_decode_attention_in_the_2_norm(dtype, wide, hq, hk, d, lens, scale):
     assert far(out.cpu()[..., keep], want, bound, dt) <= 1
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("mix", ["alone", "zeros", "flat"])
+@pytest.mark.parametrize("log_size", [-90, -60, -30, 30, 60, 100])
+def test_values_of_any_size(dtype, mix, log_size):
+    """Values from 2^-90 to 2^100 in size: alone, beside likelier positions whose values are all zero, and beside
+    flat rows (one value throughout, no codes) of the same size or of size 1."""
+    dt, hq, hk, d, n, scale = DT[dtype], 4, 2, 64, 400, 0.1
+    g = torch.Generator().manual_seed(log_size + 200)
+    k, v = (torch.randn(1, hk, n, d, generator=g) for _ in range(2))
+    q = torch.randn(1, hq, d, generator=g).to(dt)
+    v = v * 2.0 ** log_size
+    some = torch.arange(n) % 5 == 0
+    some[100:300] = True  # whole tiles and, in turn with them, single positions
+    if mix == "zeros":
+        v[:, :, some] = 0.0
+        k[:, :, some] += 3 * q.float().view(1, hk, hq // hk, d).mean(2)[:, :, None] / 8 ** 0.5
+    if mix == "flat":
+        flat = torch.randn(1, hk, n, 1, generator=g) * torch.where(torch.arange(n) % 2 == 0, 2.0 ** log_size, 1.0)[:, None]
+        v[:, :, some] = flat[:, :, some].expand(-1, -1, -1, d)
+    rec = records(k.to(dt), v.to(dt))
+    for promise, splits in ((n, 4), (130000, 1)):
+        cache = torch.zeros(1, hk, promise, d + 16, dtype=torch.uint8)
+        cache[:, :, :n] = rec
+        assert splits_of(1, hq, hk, d, promise) >= splits
+        out = ops.decode_attention_q4(q.cuda(), cache.cuda(), torch.tensor([n], dtype=torch.int32, device="cuda"), hk,
+                                      promise, scale)
+        # Weights fall below f16's 2^-14 where v_scale is below 2^-80: 2^-25 beside 2^-5 of the largest at 2^-92.
+        want, bound = attention64(q, rec, [n], scale, splits, least=2.0 ** -32 if log_size > -70 else 2.0 ** -20)
+        assert far(out.cpu(), want, bound, dt) <= 1, promise
+
+
 def emulated(q, rec, lens, scale, dt, chunk, lose=None, weights=torch.float16, centred=True, merge=True):
     """The kernel's sums with its weights rounded to `weights` times the scale, and mistakes: a lost chunk, codes
     that are not centred, parts added up without their maxima."""
