@@ -77,6 +77,7 @@ _SIGNATURES = {
                            c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_size_t,
                            c_int, c_void_p]),
     "hx_gemm_q4_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int]),
+    "hx_gemm_q4_launches": (c_int, [c_int64, c_int64, c_int64, c_int]),
     "hx_token_logprobs": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "hx_kv_pack": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,

@@ -515,6 +515,11 @@ extern "C" size_t hx_gemm_q4_workspace(int64_t m, int64_t n, int64_t k, int64_t 
   return k <= (m <= 8 ? 64 : 32) * kUnitK ? 0 : (size_t)m * n * sizeof(float);
 }
 
+extern "C" int hx_gemm_q4_launches(int64_t m, int64_t n, int64_t k, int dtype) {
+  if (m <= 0) return 0;
+  return dtype != HX_F32 && use_tc(m, n, k) ? 3 : 1;
+}
+
 extern "C" int hx_gemm_q4(const void* a, const void* w, const void* scales, void* c, int64_t m,
                           int64_t n, int64_t k, int64_t group, int64_t lda, int64_t ldc,
                           int epilogue, const void* residual, int64_t ld_residual, void* workspace,

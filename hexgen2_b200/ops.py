@@ -494,7 +494,7 @@ def gemm_q4(a, w_q4, scales, epilogue=HX_EPI_NONE, residual=None, out=None):
           K, group, a.stride(0) if M > 1 else K,
           out.stride(0) if M > 1 else cols, epilogue, _p(residual),
           0 if residual is None else residual.stride(0) if M > 1 else cols, _p(ws), nbytes, code)
-    _count(3 if M > 16 and nbytes else 1)
+    _count(_L().hx_gemm_q4_launches(M, N, K, code) if nbytes else 1)
     return out
 
 

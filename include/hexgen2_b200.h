@@ -292,6 +292,8 @@ int hx_gemm_q4(const void* a, const void* w, const void* scales, void* c, int64_
                const void* residual, int64_t ld_residual, void* workspace, size_t workspace_bytes,
                int dtype, void* stream);
 size_t hx_gemm_q4_workspace(int64_t m, int64_t n, int64_t k, int64_t group, int dtype);
+/* Kernels that hx_gemm_q4 launches for these sizes: 1, or 3 for the large products of more than 16 rows. */
+int hx_gemm_q4_launches(int64_t m, int64_t n, int64_t k, int dtype);
 
 /* ---------------------------------------------------------------- sampling */
 /* out_idx[r] = first index of the maximum of logits[r, 0:cols] (torch.argmax semantics).

@@ -166,3 +166,13 @@ def test_attention_workspace_covers_the_partials():
     assert w(0, 8, 2, 128, 100) == 0 and w(1, 8, 2, 128, 0) == 0
     assert w(1, 8, 1, 128, 100000) > 0
     assert w(1, 8, 1, 128, 100000) % 4 == 0
+
+
+@pytest.mark.parametrize("m,n,k,dtype,launches", [
+    (1, 32000, 4096, _lib.HX_BF16, 1), (16, 32000, 4096, _lib.HX_BF16, 1), (17, 32000, 4096, _lib.HX_BF16, 3),
+    (32, 4096, 4096, _lib.HX_F16, 3), (32, 4095, 4096, _lib.HX_F16, 1), (40, 40, 8448, _lib.HX_BF16, 1),
+    (64, 32000, 4096, _lib.HX_F32, 1), (0, 32000, 4096, _lib.HX_BF16, 0)])
+def test_gemm_q4_launches(m, n, k, dtype, launches):
+    """One kernel, or three on tcgen05 (2^29 products of more than 16 rows); running sums alone, which need a
+    workspace too, do not make it three."""
+    assert _lib.lib().hx_gemm_q4_launches(m, n, k, dtype) == launches

@@ -468,6 +468,17 @@ def test_gemm_q4_rows_do_not_mix():
     assert out[11].isnan().all()
 
 
+@pytest.mark.parametrize("M,N,K,launches", [(1, 64, 256, 1), (12, 64, 8448, 1), (40, 40, 8448, 1), (20, 8192, 4096, 3)])
+def test_gemm_q4_counts_its_launches(M, N, K, launches):
+    """ops.LAUNCHES grows by the kernels that a call launches; a workspace does not say how many."""
+    a = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(N, K // 2, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(N, K // 128, dtype=torch.bfloat16, device="cuda")
+    before = ops.LAUNCHES
+    ops.gemm_q4(a, w, scales)
+    assert ops.LAUNCHES - before == launches
+
+
 def test_one_row_of_any_stride():
     """A single row of a whose stride is not a multiple of 16 bytes."""
     g = torch.Generator().manual_seed(2)
