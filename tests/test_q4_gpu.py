@@ -468,6 +468,92 @@ def test_gemm_q4_rows_do_not_mix():
     assert out[11].isnan().all()
 
 
+# Small products, several passes of one kernel, running sums over k, and the tcgen05 kernels (2^29 products of 17 and more
+# rows) with 32 and 64 rows to a block.
+PATHS = [(5, 96, 256, 64), (20, 160, 512, 128), (12, 64, 8448, 128), (20, 8192, 4096, 128), (40, 4128, 4096, 64)]
+
+
+@pytest.mark.parametrize("M,N,K,group", PATHS)
+@pytest.mark.parametrize("epilogue", [0, 1, 2])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_gemm_q4_strides_and_in_place_on_every_path(dtype, epilogue, M, N, K, group):
+    """a, residual and out inside wider buffers whose neighbours are left alone, and the residual updated in place:
+    the bits of the contiguous call."""
+    dt = DT[dtype]
+    g = torch.Generator().manual_seed(M + N + epilogue)
+    cols = N // 2 if epilogue == 2 else N
+    wide = torch.full((M, K + 64), float("nan"))
+    wide[:, 32:32 + K] = torch.randn(M, K, generator=g)
+    wide = wide.to(dt).cuda()
+    a = wide[:, 32:32 + K]
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8).cuda()
+    scales = (0.02 * torch.exp(0.3 * torch.randn(N, K // group, generator=g))).to(dt).cuda()
+    res = torch.randn(M, cols + 3, generator=g).to(dt).cuda()[:, 1:1 + cols] if epilogue == 1 else None
+    want = ops.gemm_q4(a.contiguous(), codes, scales, epilogue, residual=None if res is None else res.contiguous())
+    assert want.isfinite().all()
+    room = torch.full((M, cols + 9), 3.0, dtype=dt, device="cuda")
+    ops.gemm_q4(a, codes, scales, epilogue, residual=res, out=room[:, 5:5 + cols])
+    assert torch.equal(room[:, 5:5 + cols], want)
+    assert (room[:, :5] == 3).all() and (room[:, 5 + cols:] == 3).all()
+    if epilogue == 1:
+        room[:, 5:5 + cols] = res
+        ops.gemm_q4(a, codes, scales, epilogue, residual=room[:, 5:5 + cols], out=room[:, 5:5 + cols])
+        assert torch.equal(room[:, 5:5 + cols], want)
+        assert (room[:, :5] == 3).all() and (room[:, 5 + cols:] == 3).all()
+    assert ops.device_error() == 0
+
+
+@pytest.mark.parametrize("M,N,K,group", PATHS)
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_gemm_q4_rows_with_infinities_and_nan_on_every_path(dtype, M, N, K, group):
+    """A row of a with an infinity or NaN gives NaN in all of its own row, and nothing in another."""
+    dt = DT[dtype]
+    g = torch.Generator().manual_seed(N)
+    a = torch.randn(M, K, generator=g).to(dt).cuda()
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8).cuda()
+    scales = (0.02 * torch.exp(0.3 * torch.randn(N, K // group, generator=g))).to(dt).cuda()
+    bad = a.clone()
+    rows = {0: float("inf"), 2: float("-inf"), M - 1: float("nan")}
+    for r, x in rows.items():
+        bad[r, (r * 37 + 100) % K] = x
+    keep = [i for i in range(M) if i not in rows]
+    for epilogue in (0, 2):
+        clean, out = (ops.gemm_q4(x, codes, scales, epilogue) for x in (a, bad))
+        assert torch.equal(out[keep], clean[keep])
+        assert out[list(rows)].isnan().all()
+
+
+@pytest.mark.parametrize("M,N,K,group", PATHS)
+def test_gemm_q4_in_graphs_and_on_streams(M, N, K, group):
+    """Two captured graphs and eager calls on a side stream at once, each with scratch of its own, give the
+    eager results whichever order they run in."""
+    dt = torch.bfloat16
+    g = torch.Generator().manual_seed(K)
+    xs = [torch.randn(M, K, generator=g).to(dt).cuda() for _ in range(3)]
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, dtype=torch.uint8).cuda()
+    scales = (0.02 * torch.exp(0.3 * torch.randn(N, K // group, generator=g))).to(dt).cuda()
+    want = [ops.gemm_q4(x, codes, scales, ops.HX_EPI_SWIGLU) for x in xs]
+    graphs, outs = [], []
+    for x in xs[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.gemm_q4(x, codes, scales, ops.HX_EPI_SWIGLU))
+        graphs.append(graph)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        graphs[1].replay()
+        with torch.cuda.stream(side):
+            graphs[0].replay()
+            third = ops.gemm_q4(xs[2], codes, scales, ops.HX_EPI_SWIGLU)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(third, want[2])
+    assert ops.device_error() == 0
+
+
 @pytest.mark.parametrize("M,N,K,launches", [(1, 64, 256, 1), (12, 64, 8448, 1), (40, 40, 8448, 1), (20, 8192, 4096, 3)])
 def test_gemm_q4_counts_its_launches(M, N, K, launches):
     """ops.LAUNCHES grows by the kernels that a call launches; a workspace does not say how many."""
