@@ -349,7 +349,7 @@ def _check_rows(what, cache):
     if cache.dim() != 5 or cache.shape[2] != 2:
         raise ValueError(f"{what}: cache must be [batch, rows, 2, kv heads, head_dim]")
     hk, d = cache.shape[3:]
-    if cache.stride()[2:] != (hk * d, d, 1):
+    if cache.stride(2) != hk * d or (cache.stride(3) != d and hk > 1) or cache.stride(4) != 1:
         raise ValueError(f"{what}: the values of a cache row must be contiguous")
     return hk, d
 
@@ -430,7 +430,7 @@ def decode_attention_q4(q, cache_q4, seqlens, n_heads_kv, max_seqlen, softmax_sc
     """decode_attention over a 4-bit cache: q [B, hq, d] against the first seqlens[b] records of
     cache_q4[b] (seqlens int32 on device, each at most max_seqlen; 0 gives zeros)."""
     what = "decode_attention_q4"
-    if q.dim() != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+    if q.dim() != 3 or q.stride(2) != 1 or (q.stride(1) != q.shape[2] and q.shape[1] > 1):
         raise ValueError(f"{what}: q must be [batch, n_heads, head_dim] with contiguous heads")
     B, hq, d = q.shape
     _check_q4(what, cache_q4, n_heads_kv, d, 0, B)
@@ -447,7 +447,7 @@ def decode_attention_q4(q, cache_q4, seqlens, n_heads_kv, max_seqlen, softmax_sc
     nbytes = decode_q4_workspace_bytes(B, hq, n_heads_kv, d, max_seqlen)
     # A buffer of its own for every call: calls on several streams, and graphs, do not share it.
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _call(dev, _L().hx_decode_attention_q4, q.data_ptr(), q.stride(0), cache_q4.data_ptr(),
+    _call(dev, _L().hx_decode_attention_q4, q.data_ptr(), q.stride(0) if B > 1 else hq * d, cache_q4.data_ptr(),
           cache_q4.stride(0), cache_q4.stride(1), seqlens.data_ptr(), B, hq, n_heads_kv, d,
           max_seqlen, float(softmax_scale), out.data_ptr(), _p(ws), nbytes, _code(q))
     _count(2 if nbytes else 1)

@@ -316,6 +316,32 @@ def test_decode_attention_nan_and_strides():
     assert torch.equal(shared, alone) and ops.device_error() == 0
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_decode_attention_sizes_of_one_have_any_stride(dtype):
+    """One query, and one head per sequence, whose strides torch leaves open."""
+    dt, d = DT[dtype], 64
+    g = torch.Generator().manual_seed(12)
+    rec = make_cache(3, 1, 40, d, g, dt, 0.3).cuda()
+    wide = torch.randn(1, 4 * d + 3, generator=g).to(dt).cuda()
+    q = wide[:, :4 * d].view(1, 4, d)  # 4 d + 3 elements from one sequence to the next
+    run = lambda q, n: ops.decode_attention_q4(q, rec[:n], i32([40, 7, 33][:n]), 1, 40, 0.1)  # noqa: E731
+    assert torch.equal(run(q, 1), run(q.contiguous(), 1))
+    q = torch.randn(1, 3, d, generator=g).to(dt).cuda().transpose(0, 1)  # heads 3 d apart, contiguous all the same
+    assert q.stride(1) != d and torch.equal(run(q, 3), run(q.clone(memory_format=torch.contiguous_format), 3))
+
+
+def test_records_of_one_head_of_any_stride():
+    """Rows [batch, rows, 2, 1, d] of a single KV head, 2 d apart as torch has it."""
+    d, n = 64, i32([5, 3])
+    rows = torch.randn(2, 5, 1, 2, d, device="cuda").transpose(2, 3)
+    assert rows.is_contiguous() and rows.stride(3) != d
+    q4 = ops.quantize_cache_q4(rows, n, ops.allocate_cache_q4(2, 1, 5, d).zero_())
+    assert torch.equal(q4, ops.quantize_cache_q4(rows.clone(memory_format=torch.contiguous_format), n, torch.zeros_like(q4)))
+    back = ops.dequantize_cache_q4(q4, n, torch.zeros_like(rows))
+    assert torch.equal(back, ops.dequantize_cache_q4(q4, n, torch.zeros(2, 5, 2, 1, d, device="cuda")))
+    assert ops.device_error() == 0
+
+
 def test_decode_attention_lengths_beyond_the_promise():
     dt, d = torch.bfloat16, 128
     g = torch.Generator().manual_seed(3)
