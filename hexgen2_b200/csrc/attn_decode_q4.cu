@@ -200,15 +200,6 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
 constexpr int kTile = 32;    // positions per stage
 constexpr int kStages = 4;
 
-HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                       const uint32_t (&b)[2]) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
-}
-
 // Transpose of the 8x8 16-bit matrix that a warp holds one row pair per lane.
 HX_DEVICE uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -220,14 +211,6 @@ HX_DEVICE float lg2_approx(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-HX_DEVICE void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_u32(smem_dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
 }
 
 template <int D, int NT>
@@ -295,7 +278,7 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           mma_f16(s[sub][nt], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u,
-                  qf[nt][2 * w + h]);
+                  qf[nt][2 * w + h][0], qf[nt][2 * w + h][1]);
       }
   }
   // Scores in base 2, and the tile's largest score + log2 v_scale per head.
@@ -399,9 +382,9 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
       const uint32_t y = __byte_perm(vw[2][i / 4], vw[3][i / 4], sel);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        mma_f16(st.o[nt][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, bh[nt]);
+        mma_f16(st.o[nt][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, bh[nt][0], bh[nt][1]);
         if (kTwo)
-          mma_f16(st.o[nt][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, bl[nt]);
+          mma_f16(st.o[nt][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, bl[nt][0], bl[nt][1]);
       }
     }
   }

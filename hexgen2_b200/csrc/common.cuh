@@ -230,6 +230,15 @@ HX_DEVICE void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar
       : "memory");
 }
 
+// Untiled copy to this CTA's shared memory: both addresses 16-byte aligned, a multiple of 16 bytes.
+HX_DEVICE void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 HX_DEVICE void prefetch_tensormap(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -412,6 +421,15 @@ inline int allow_shared(const void* kern, int bytes, std::atomic<uint64_t>& allo
 // ---------------------------------------------------------------------------------------
 // Small math helpers
 // ---------------------------------------------------------------------------------------
+// c += A (16 x 16, f16) * B (16 x 8, f16) by a warp, f32 sums.
+HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 HX_DEVICE float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

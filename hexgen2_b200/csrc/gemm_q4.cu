@@ -120,14 +120,6 @@ struct Block {
   static constexpr int kPartial = kWarps * NT * 8 * 16;  // floats
 };
 
-HX_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // Largest |x| of eight 16-bit floats, as its bits (NaN above infinity above the rest).
 HX_DEVICE uint32_t largest_bits(uint4 v) {
   const uint32_t m = 0x7fff7fffu;
@@ -239,14 +231,6 @@ HX_DEVICE void multiply(const uint8_t* w, const float (&s)[2][kPair * (kUnitK / 
       }
     }
   }
-}
-
-HX_DEVICE void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_u32(smem_dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
 }
 
 #include "gemm_q4_tc.cuh"

@@ -1,4 +1,5 @@
-// gemm_q4 on tcgen05: large weights times 17 to 64 rows of a (gemm_q4.cu has the operator and its other kernels).
+// gemm_q4 on tcgen05: large weights times 17 to 64 rows of a. A part of gemm_q4.cu, which has the operator, its
+// other kernels and the arguments and conversions that both use, and includes this once.
 //
 // D[128 weight rows, NT rows of a] = A B^T by tcgen05.mma kind::f16, M = 128. A, the codes, is made in tensor
 // memory: the bits of a code are an f16 as they stand (codes * 2^-24, or 2^-20 one nibble up), so a
