@@ -157,3 +157,14 @@ def test_logits_masked_with_low_finite_values(dtype, mask, rows, vocab):
     got = ops.token_logprobs(x.cuda(), tokens.cuda(), top_k=5, entropy=True)
     assert got.entropy.isfinite().all() and got.logprobs.isfinite().all()
     check(x, tokens, 5, got)
+
+
+def test_rows_beyond_32_bits():
+    """Logits of more than 2^32 bytes and 2^31 elements: the last rows as in a small batch."""
+    rows, vocab = 17000, 131077
+    x = torch.zeros(rows, vocab, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(3)
+    x[-3:] = torch.randn(3, vocab, generator=g).bfloat16().cuda()
+    tokens = torch.full((rows,), vocab - 1, device="cuda")
+    got = ops.token_logprobs(x, tokens, top_k=4, entropy=True)
+    check(x[-3:].cpu(), tokens[-3:].cpu(), 4, ops.TokenLogprobs(*(t[-3:] for t in got)))

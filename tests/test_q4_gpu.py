@@ -618,6 +618,63 @@ def test_an_error_left_by_another_call_spoils_nothing():
     assert ops.device_error() == 2
 
 
+# ------------------------------------------------------------------------------ far offsets
+def test_offsets_beyond_32_bits():
+    """Caches of more than 2^32 bytes and 2^31 elements: rows near the end of the last sequence become records near the
+    end of the last sequence and head, are attended to and read back as in a small cache."""
+    d, hk, n, S = 128, 2, 5, 1 << 23
+    dt = torch.bfloat16
+    g = torch.Generator().manual_seed(31)
+    rows = torch.randn(1, n, 2, hk, d, generator=g).to(dt).cuda()
+    far = torch.empty(3, 1 << 22, 2, hk, d, dtype=dt, device="cuda")  # 2^31 elements a sequence
+    far[2, :n] = rows[0]
+    far[2, -n:] = rows[0].flip(0)
+    small, big = ops.allocate_cache_q4(1, hk, n, d), ops.allocate_cache_q4(4, hk, S, d)  # 2.4e9 bytes a sequence
+    ops.quantize_cache_q4(rows, i32([n]), small)
+    big[3, :, :n], big[3, :, -n:] = 0x77, 0x77
+    ops.quantize_cache_q4(far, i32([0, 0, n]), big, starts=i32([0, 0, S - n]), batch_offset=1)
+    assert torch.equal(big[3, :, S - n:], small[0]) and (big[3, :, :n] == 0x77).all()
+    back = ops.dequantize_cache_q4(small, i32([n]), torch.zeros_like(rows))
+    far[2, :n] = 0
+    ops.dequantize_cache_q4(big, i32([0, 0, n]), far, starts=i32([0, 0, S - n]), batch_offset=1)
+    assert torch.equal(far[2, :n], back[0])
+    # All rows of a sequence: the last ones lie beyond 2^31 elements.
+    ops.quantize_cache_q4(far[2:], i32([1 << 22]), big, batch_offset=3)
+    assert torch.equal(big[3, :, (1 << 22) - n:1 << 22].flip(1), small[0])
+    q = torch.randn(1, 4, d, generator=g).to(dt).cuda()
+    ops.quantize_cache_q4(rows, i32([n]), big, batch_offset=3)
+    assert torch.equal(ops.decode_attention_q4(q, big[3:], i32([n]), hk, n, 0.1),
+                       ops.decode_attention_q4(q, small, i32([n]), hk, n, 0.1))
+    # The last record of the longest sequence takes all of the probability.
+    big[3].zero_()
+    spike = torch.zeros(1, 1, 2, hk, d, dtype=dt, device="cuda")
+    spike[:, :, 0] = 30 * q.view(1, 1, hk, 2, d).sum(3)
+    spike[:, :, 1] = rows[:, :1, 1]
+    ops.quantize_cache_q4(spike, i32([1]), big, starts=i32([S - 1]), batch_offset=3)
+    last = ops.allocate_cache_q4(1, hk, 1, d)
+    ops.quantize_cache_q4(spike, i32([1]), last)
+    out = ops.decode_attention_q4(q, big[3:], i32([S]), hk, S, 1.0)
+    assert torch.equal(out, ops.decode_attention_q4(q, last, i32([1]), hk, 1, 1.0)) and ops.device_error() == 0
+
+
+@pytest.mark.parametrize("M", [3, 40])
+def test_gemm_q4_weights_beyond_32_bits(M):
+    """A weight of more than 2^32 bytes: its last rows against 64 bits."""
+    N, K, n = (1 << 20) + 128, 8192, 256
+    g = torch.Generator().manual_seed(M)
+    w = torch.full((N, K // 2), 0x88, dtype=torch.uint8, device="cuda")
+    w[-n:] = torch.randint(0, 256, (n, K // 2), generator=g, dtype=torch.uint8).cuda()
+    scales = torch.ones(N, K // 128, dtype=torch.bfloat16, device="cuda")
+    a = torch.randn(M, K, generator=g).bfloat16().cuda()
+    out = ops.gemm_q4(a, w, scales)
+    want, bound = linear64(a.cpu(), w[-n:].cpu(), scales[-n:].cpu(), 0, None)
+    off = (out[:, -n:].cpu().double() - want).abs()
+    assert (off <= want.abs() * half_step(torch.bfloat16) * 1.01 + bound).all()
+    # Weights of 0 (code 8) and the scales of the rows above: f32 sums of a's share of the codes and of their offset,
+    # which cancel up to the same bound.
+    assert (out[:, :-n].abs().amax(1).cpu().double() <= bound[:, 0]).all() and ops.device_error() == 0
+
+
 # ------------------------------------------------------------------------------ together
 def layer(x, res, w, cos, sin, q4, pos, seqlens, hq, hk, d, cap, head):
     """One decode step of one layer and the LM head, in 4 bits."""
