@@ -184,7 +184,12 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
 //     2^-25 * 2^-7 of the largest. So that this moves a value's distance from the middle of its row and not
 //     its codes, which are many times the output where values average out, the codes are taken about 7.5:
 //     the rounded P' times 7.5 go off again in f32, the middle v_min + 7.5 v_scale comes in with p itself.
-//     For f16 outputs, whose half step is no coarser, P' is the sum of two f16 (2^-22).
+//   - For f16 outputs, whose half step is no coarser, P' is the sum of two f16 (2^-22), and what the tensor core
+//     cuts off its sums counts too. It cuts towards zero: codes in place of signed values made 20000
+//     positions 2e-4 of the output too low. So the sum of 7.5 P' is the tensor core's as well, cut alike (the mean
+//     of eight rows of codes 6 to 9), and no code lies below bit 4: as measured, products are cut at about
+//     2^-24 of the largest with a subnormal operand counted as 2^-14, so codes in the lowest bits had 14 bits
+//     left. (bf16 rounds eight times as much off and does without both, 7 % of its time.)
 //   - S comes out position-major; movmatrix turns it into the B operand of O.
 // Each warp streams 32-position tiles through a ring of its own (bulk copies by its lane 0, one
 // mbarrier per stage): no block barrier until the warps' partials are added up at the end.
@@ -222,11 +227,11 @@ struct McSmem {
 
 // State of one warp's online softmax. Per lane, for columns 2t + j of each tile of eight: the
 // reference r (the same in all lanes of equal t), this lane's shares of sum p and of what all output elements
-// have in common (z: sum p v_min, or p times the rows' middles less 7.5 sum P'), and the output elements of
-// its rows, even elements times 2^-24, odd ones times 2^-20.
+// have in common (z: p times the rows' middles; bf16: less 7.5 P'), and the output elements of its rows times
+// 2^-20 (bf16: even elements times 2^-24). f16: c, the output of rows of codes 6, 6, 7, 7, 8, 8, 9, 9, times 2^-20.
 template <int D, int NT, int NJ>
 struct Softmax {
-  float r[NT][NJ], l[NT][NJ], z[NT][NJ], o[NT][D / 16][4];
+  float r[NT][NJ], l[NT][NJ], z[NT][NJ], o[NT][D / 16][4], c[NT][4];
 };
 
 // What the reference follows of a row's values is log2 of v_scale, or of 2^-24 |v_min| where that is more (flat rows,
@@ -328,6 +333,7 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
         st.z[nt][j] *= f;
 #pragma unroll
         for (int i = 0; i < OT; ++i) st.o[nt][i][j] *= f, st.o[nt][i][2 + j] *= f;
+        if (kTwo) st.c[nt][j] *= f;
       }
   }
 #pragma unroll
@@ -338,14 +344,14 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const bool live = kFull || sub * 16 + r * 8 + g < n;  // stale scales may be NaN
-        const float base = kTwo ? meta[sub][r].w : fmaf(7.5f, meta[sub][r].z, meta[sub][r].w);
+        const float middle = fmaf(7.5f, meta[sub][r].z, meta[sub][r].w);
         float pv[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
           const float p = ex2_approx(s[sub][nt][2 * r + j] - st.r[nt][j]);
           if (live) {
             st.l[nt][j] += p;
-            st.z[nt][j] = fmaf(p, base, st.z[nt][j]);
+            st.z[nt][j] = fmaf(p, middle, st.z[nt][j]);
             pv[j] = p * meta[sub][r].z;
           }
         }
@@ -359,6 +365,14 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
           if constexpr (NJ == 2) st.z[nt][1] = fmaf(-7.5f, back.y, st.z[nt][1]);
         }
       }
+    if constexpr (kTwo) {
+      const uint32_t same = (6 + g / 2) * 0x00100010u;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        mma_f16(st.c[nt], same, same, same, same, bh[nt][0], bh[nt][1]);
+        mma_f16(st.c[nt], same, same, same, same, bl[nt][0], bl[nt][1]);
+      }
+    }
     // V codes of positions 2t, 2t + 1, 2t + 8, 2t + 9: lane (g, t) takes bytes [D/16 g, D/16 (g + 1)).
     const uint8_t* v = tile + (sub * 16 + 2 * t) * kRec + D / 2 + (D / 16) * g;
     constexpr int VW = D >= 64 ? D / 64 : 1;
@@ -380,11 +394,12 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
       const uint32_t sel = (i % 4) * 0x0011u + (4 + i % 4) * 0x1100u;
       const uint32_t x = __byte_perm(vw[0][i / 4], vw[1][i / 4], sel);
       const uint32_t y = __byte_perm(vw[2][i / 4], vw[3][i / 4], sel);
+      const uint32_t x0 = kTwo ? (x * 16u) & 0x00f000f0u : x & 0x000f000fu, x1 = x & 0x00f000f0u;
+      const uint32_t y0 = kTwo ? (y * 16u) & 0x00f000f0u : y & 0x000f000fu, y1 = y & 0x00f000f0u;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        mma_f16(st.o[nt][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, bh[nt][0], bh[nt][1]);
-        if (kTwo)
-          mma_f16(st.o[nt][i], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, bl[nt][0], bl[nt][1]);
+        mma_f16(st.o[nt][i], x0, x1, y0, y1, bh[nt][0], bh[nt][1]);
+        if (kTwo) mma_f16(st.o[nt][i], x0, x1, y0, y1, bl[nt][0], bl[nt][1]);
       }
     }
   }
@@ -394,6 +409,7 @@ template <typename T, int D, int NT, int NJ>
 __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
   constexpr int kRec = D + 16, W = D / 32, OT = D / 16;
   constexpr int kHeads = NT * 4 * NJ;  // head h sits in column h (NJ = 2) or 2h (NJ = 1)
+  constexpr bool kTwo = std::is_same<T, __half>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[kWarps][kStages];
   __shared__ float sm_m[kWarps][kHeads], sm_l[kWarps][kHeads];
@@ -490,6 +506,8 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
     for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) st.o[nt][i][j] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) st.c[nt][j] = 0.f;
   }
 
   int done = 0;
@@ -518,6 +536,7 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
       for (int x = 4; x < 32; x <<= 1) {
         st.l[nt][j] += __shfl_xor_sync(0xffffffffu, st.l[nt][j], x);
         st.z[nt][j] += __shfl_xor_sync(0xffffffffu, st.z[nt][j], x);
+        if (kTwo) st.c[nt][j] += __shfl_xor_sync(0xffffffffu, st.c[nt][j], x);
       }
       const int h = (nt * 4 + t) * NJ + j;
       if (g == 0) sm_m[warp][h] = st.r[nt][j], sm_l[warp][h] = st.l[nt][j];
@@ -531,8 +550,10 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
         *reinterpret_cast<float2*>(sm_o + (warp * kHeads + (nt * 4 + t) * NJ + j) * D + (D / 8) * g + 2 * i) =
-            make_float2(fmaf(st.o[nt][i][j], 16777216.f, st.z[nt][j]),
-                        fmaf(st.o[nt][i][2 + j], 1048576.f, st.z[nt][j]));
+            kTwo ? make_float2(fmaf(st.o[nt][i][j] - 0.125f * st.c[nt][j], 1048576.f, st.z[nt][j]),
+                               fmaf(st.o[nt][i][2 + j] - 0.125f * st.c[nt][j], 1048576.f, st.z[nt][j]))
+                 : make_float2(fmaf(st.o[nt][i][j], 16777216.f, st.z[nt][j]),
+                               fmaf(st.o[nt][i][2 + j], 1048576.f, st.z[nt][j]));
   __syncthreads();
   for (int i = tid; i < nq * D; i += kThreads) {
     const int q = i / D;
