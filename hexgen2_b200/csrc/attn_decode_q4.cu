@@ -181,15 +181,15 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
 //     a position's V codes (bytes of two positions joined with one permute).
 //   - P' enters as f16, relative to the largest P' seen (the running reference r follows
 //     s + log2 v_scale, not s, down to v_scale = 2^-80): at most 2^-11 of each value off, and
-//     2^-25 * 2^-7 of the largest. So that this moves a value's distance from the middle of its row and not
-//     its codes, which are many times the output where values average out, the codes are taken about 7.5:
-//     the rounded P' times 7.5 go off again in f32, the middle v_min + 7.5 v_scale comes in with p itself.
-//   - For f16 outputs, whose half step is no coarser, P' is the sum of two f16 (2^-22), and what the tensor core
-//     cuts off its sums counts too. It cuts towards zero: codes in place of signed values made 20000
-//     positions 2e-4 of the output too low. So the sum of 7.5 P' is the tensor core's as well, cut alike (the mean
-//     of eight rows of codes 6 to 9), and no code lies below bit 4: as measured, products are cut at about
-//     2^-24 of the largest with a subnormal operand counted as 2^-14, so codes in the lowest bits had 14 bits
-//     left. (bf16 rounds eight times as much off and does without both, 7 % of its time.)
+//     2^-25 * 2^-7 of the largest. For f16 outputs, whose half step is no coarser, P' is the sum of two f16 (2^-22).
+//   - Where values average out, sums of codes are many times the output, and so would be what they lose: the
+//     rounding of P', and what the tensor core cuts off its sums, always towards zero (of 20000 positions 2e-4
+//     of the output). So codes are taken about 7.5: the sum of 7.5 P' that goes off is the tensor core's own,
+//     rounded and cut alike (the mean of eight rows of codes 6 to 9), and a row's middle v_min + 7.5 v_scale
+//     comes in with p itself, in f32.
+//   - As measured, products are cut at about 2^-24 of the largest with a subnormal operand counted as 2^-14, so
+//     a code in the lowest bits keeps 14. For f16 outputs, even elements move to bit 4 and up as well (bf16 rounds
+//     eight times as much off and does without, 5 % of its time).
 //   - S comes out position-major; movmatrix turns it into the B operand of O.
 // Each warp streams 32-position tiles through a ring of its own (bulk copies by its lane 0, one
 // mbarrier per stage): no block barrier until the warps' partials are added up at the end.
@@ -226,9 +226,9 @@ struct McSmem {
 };
 
 // State of one warp's online softmax. Per lane, for columns 2t + j of each tile of eight: the
-// reference r (the same in all lanes of equal t), this lane's shares of sum p and of what all output elements
-// have in common (z: p times the rows' middles; bf16: less 7.5 P'), and the output elements of its rows times
-// 2^-20 (bf16: even elements times 2^-24). f16: c, the output of rows of codes 6, 6, 7, 7, 8, 8, 9, 9, times 2^-20.
+// reference r (the same in all lanes of equal t), this lane's shares of sum p and of the sum of p times the rows'
+// middles (z), the output elements of its rows times 2^-20 (bf16: even elements times 2^-24), and c, the
+// outputs of rows of codes 6, 6, 7, 7, 8, 8, 9, 9 as the even and the odd elements hold them (f16: one for both).
 template <int D, int NT, int NJ>
 struct Softmax {
   float r[NT][NJ], l[NT][NJ], z[NT][NJ], o[NT][D / 16][4], c[NT][4];
@@ -333,7 +333,8 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
         st.z[nt][j] *= f;
 #pragma unroll
         for (int i = 0; i < OT; ++i) st.o[nt][i][j] *= f, st.o[nt][i][2 + j] *= f;
-        if (kTwo) st.c[nt][j] *= f;
+        st.c[nt][j] *= f;
+        if (!kTwo) st.c[nt][2 + j] *= f;
       }
   }
 #pragma unroll
@@ -357,21 +358,16 @@ HX_DEVICE void attend_tile(const uint8_t* tile, int n, float scale_log2, const u
         }
         const uint32_t hi = pack2<__half>(pv[0], pv[1]);
         bh[nt][r] = transpose8x8(hi);
-        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
         if constexpr (kTwo) {
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
           bl[nt][r] = transpose8x8(pack2<__half>(pv[0] - back.x, pv[1] - back.y));
-        } else {
-          st.z[nt][0] = fmaf(-7.5f, back.x, st.z[nt][0]);
-          if constexpr (NJ == 2) st.z[nt][1] = fmaf(-7.5f, back.y, st.z[nt][1]);
         }
       }
-    if constexpr (kTwo) {
-      const uint32_t same = (6 + g / 2) * 0x00100010u;
+    const uint32_t odd = (6 + g / 2) * 0x00100010u, even = kTwo ? odd : odd >> 4;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        mma_f16(st.c[nt], same, same, same, same, bh[nt][0], bh[nt][1]);
-        mma_f16(st.c[nt], same, same, same, same, bl[nt][0], bl[nt][1]);
-      }
+    for (int nt = 0; nt < NT; ++nt) {
+      mma_f16(st.c[nt], even, odd, even, odd, bh[nt][0], bh[nt][1]);
+      if (kTwo) mma_f16(st.c[nt], even, odd, even, odd, bl[nt][0], bl[nt][1]);
     }
     // V codes of positions 2t, 2t + 1, 2t + 8, 2t + 9: lane (g, t) takes bytes [D/16 g, D/16 (g + 1)).
     const uint8_t* v = tile + (sub * 16 + 2 * t) * kRec + D / 2 + (D / 16) * g;
@@ -536,7 +532,8 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
       for (int x = 4; x < 32; x <<= 1) {
         st.l[nt][j] += __shfl_xor_sync(0xffffffffu, st.l[nt][j], x);
         st.z[nt][j] += __shfl_xor_sync(0xffffffffu, st.z[nt][j], x);
-        if (kTwo) st.c[nt][j] += __shfl_xor_sync(0xffffffffu, st.c[nt][j], x);
+        st.c[nt][j] += __shfl_xor_sync(0xffffffffu, st.c[nt][j], x);
+        if (!kTwo) st.c[nt][2 + j] += __shfl_xor_sync(0xffffffffu, st.c[nt][2 + j], x);
       }
       const int h = (nt * 4 + t) * NJ + j;
       if (g == 0) sm_m[warp][h] = st.r[nt][j], sm_l[warp][h] = st.l[nt][j];
@@ -550,10 +547,8 @@ __global__ void __launch_bounds__(kThreads) decode_q4_mma_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
         *reinterpret_cast<float2*>(sm_o + (warp * kHeads + (nt * 4 + t) * NJ + j) * D + (D / 8) * g + 2 * i) =
-            kTwo ? make_float2(fmaf(st.o[nt][i][j] - 0.125f * st.c[nt][j], 1048576.f, st.z[nt][j]),
-                               fmaf(st.o[nt][i][2 + j] - 0.125f * st.c[nt][j], 1048576.f, st.z[nt][j]))
-                 : make_float2(fmaf(st.o[nt][i][j], 16777216.f, st.z[nt][j]),
-                               fmaf(st.o[nt][i][2 + j], 1048576.f, st.z[nt][j]));
+            make_float2(fmaf(st.o[nt][i][j] - 0.125f * st.c[nt][j], kTwo ? 1048576.f : 16777216.f, st.z[nt][j]),
+                        fmaf(st.o[nt][i][2 + j] - 0.125f * st.c[nt][kTwo ? j : 2 + j], 1048576.f, st.z[nt][j]));
   __syncthreads();
   for (int i = tid; i < nq * D; i += kThreads) {
     const int q = i / D;
