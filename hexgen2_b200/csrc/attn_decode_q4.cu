@@ -38,7 +38,10 @@ struct Args {
 
 // CUDA-core kernel: f32 products for every type. One CTA per (key split, KV head and eight of its
 // query heads, sequence); a warp takes 32 keys at a time, one per lane for the scores, all lanes
-// across D for the values.
+// across D for the values. Codes are taken about the code of zero (the nearest, where a row has no zero), so that
+// sums of products are of the values' size, not of the codes', and lose no more than plain f32 sums do.
+HX_DEVICE float code_of_zero(float scale, float low) { return scale > 0.f ? fminf(fmaxf(-low / scale, 0.f), 15.f) : 0.f; }
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
   constexpr int EPL = D / 32;  // output elements per lane
@@ -86,6 +89,8 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
     const bool valid = lane < n;
     const uint8_t* rec = recs + (int64_t)(base + (valid ? lane : 0)) * (D + 16);
     const float4 meta = *reinterpret_cast<const float4*>(rec + D);
+    const float k_zero = code_of_zero(meta.x, meta.y), k_base = fmaf(meta.x, k_zero, meta.y);
+    const float v_zero = code_of_zero(meta.z, meta.w), v_base = fmaf(meta.z, v_zero, meta.w);
     float s[NQ];
 #pragma unroll
     for (int g = 0; g < NQ; ++g) s[g] = 0.f;
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
       const uint32_t w = *reinterpret_cast<const uint32_t*>(rec + c * 4);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float code = (float)((w >> (4 * i)) & 15u);
+        const float code = (float)((w >> (4 * i)) & 15u) - k_zero;
 #pragma unroll
         for (int g = 0; g < NQ; ++g) s[g] = fmaf(sm_q[g][c * 8 + i], code, s[g]);
       }
@@ -102,19 +107,20 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
     float pv[NQ];
 #pragma unroll
     for (int g = 0; g < NQ; ++g) {
-      const float score = a.scale_log2 * (meta.x * s[g] + meta.y * sm_sum[g]);
+      const float score = a.scale_log2 * (meta.x * s[g] + k_base * sm_sum[g]);
       const float top = fmaxf(m[g], warp_max(valid ? score : -INFINITY));
       const float alpha = exp2f(m[g] - top);
       const float p = valid ? exp2f(score - top) : 0.f;
       m[g] = top;
       l[g] = l[g] * alpha + p;  // this lane's share; lanes are added up at the end
-      z[g] = z[g] * alpha + (valid ? p * meta.w : 0.f);
+      z[g] = z[g] * alpha + (valid ? p * v_base : 0.f);
       pv[g] = valid ? p * meta.z : 0.f;
 #pragma unroll
       for (int e = 0; e < EPL; ++e) o[g][e] *= alpha;
     }
     const uint8_t* vrow = recs + (int64_t)base * (D + 16) + D / 2;
     for (int j = 0; j < n; ++j, vrow += D + 16) {
+      const float zero = __shfl_sync(0xffffffffu, v_zero, j);
       float code[EPL];
       if constexpr (EPL == 1) {
         code[0] = (float)((vrow[lane >> 1] >> (4 * (lane & 1))) & 15);
@@ -126,6 +132,8 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) code[e] = (float)((w >> (4 * e)) & 15u);
       }
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) code[e] -= zero;
 #pragma unroll
       for (int g = 0; g < NQ; ++g) {
         const float w = __shfl_sync(0xffffffffu, pv[g], j);

@@ -115,7 +115,7 @@ def test_the_bound_bites(hq, hk, d, lens, scale):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("hq,hk,d,n,scale", [(1, 1, 128, 200000, 128 ** -0.5), (8, 1, 64, 65536, 0.125), (32, 4, 128, 30000, 0.05),
                                             (4, 4, 32, 100001, 0.1), (64, 64, 128, 20000, 0.0)])
 def test_long_sequences_keep_the_digits_of_their_type(dtype, hq, hk, d, n, scale):
@@ -134,4 +134,7 @@ def test_long_sequences_keep_the_digits_of_their_type(dtype, hq, hk, d, n, scale
         mine = slice(h * hq // hk, (h + 1) * hq // hk)
         want[mine] = torch.softmax(scale * (q[0, mine].double() @ (km + ks * kc).t()), -1) @ (vm + vs * vc)
     off, rounding = (out[0].double() - want).norm(), (want.to(dt).double() - want).norm()
-    assert off <= 1.12 * rounding, (off / rounding).item()
+    if dtype == "f32":  # scores and exponentials within 2^-21, sums of distances from the rows' middles
+        assert off <= 2.0 ** -19 * want.norm(), (off / want.norm()).item()
+    else:
+        assert off <= 1.12 * rounding, (off / rounding).item()
