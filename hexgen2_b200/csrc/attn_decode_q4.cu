@@ -203,10 +203,10 @@ __global__ void __launch_bounds__(kThreads) decode_q4_kernel(const Args a) {
 // mbarrier per stage): no block barrier until the warps' partials are added up at the end.
 // NT tiles of eight columns; NJ = 1 puts at most four heads into the even columns, which halves the
 // softmax work per position.
-// Measured (bf16, D = 128): 32 sequences of up to 2478 positions, 32 heads, 190 MB of records, 47 us
-// (4.0 TB/s, 0.62 of the measured copy rate); 4 documents of up to 65536, 64 heads on 8, 205 MB, 45 us
-// (4.5 TB/s, 0.69). What bounds it: instructions per position (229 per warp and 16 positions, of
-// which 88 unpack codes on the half-rate ALU pipe) at twelve warps an SM, and uneven CTAs at ragged
+// Measured (bf16, D = 128): 32 sequences of up to 2478 positions, 32 heads, 190 MB of records, 46.5 us
+// (4.1 TB/s, 0.62 of the measured copy rate; f16 53.6 us); 4 documents of up to 65536, 64 heads on 8, 205 MB,
+// 50 us (4.1 TB/s, 0.63; f16 55.7 us). What bounds it: instructions per position (225 per warp and 16
+// positions, of which 88 unpack codes on the half-rate ALU pipe) at twelve warps an SM, and uneven CTAs at ragged
 // lengths. An equal split over persistent CTAs was slower (59 and 50 us): many short runs leave some
 // CTAs with a run's fixed cost twenty times over.
 // ------------------------------------------------------------------------------------------

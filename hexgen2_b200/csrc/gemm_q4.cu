@@ -84,7 +84,9 @@ __global__ void __launch_bounds__(kThreads) gemm_q4_kernel(const Args p) {
 //     8 that codes are offset by comes off with the group's sum of a, in f32.
 //   - a goes in as f16 times a power of two of its own per (row, 128 k): max |a| in [2^9, 2^10), times 16
 //     where the codes are not, so bf16 and f16 values down to 2^-24 of the unit's largest are exact
-//     (smaller ones to 2^-35 of it). The factor comes off with the group's scale.
+//     (smaller ones to 2^-35 of it). The factor comes off with the group's scale. Products are cut, towards zero,
+//     at about 2^-14 of the largest times 1 (codes in the lowest bits): beside the rounding of an f16 output nothing,
+//     but for rows of one sign with outliers, 1.19 times its error at 300 times the rest and 16384 k.
 //   - A unit is 16 weight rows x 128 k. Nibbles 16 bits apart make one operand register, and the order of
 //     k inside a group is free, so a lane takes whole words of its two rows (16 bytes at groups of 128).
 //   - The weights are what has to move, so a stays: a CTA keeps up to 16 rows of a over up to 4096 k (8
@@ -100,7 +102,7 @@ __global__ void __launch_bounds__(kThreads) gemm_q4_kernel(const Args p) {
 //   busy at a quarter of the memory's bandwidth; bulk copies of 128 bytes took about 20 cycles each.
 //   Measured (device time): 1x4096x4096 6 us, 1x12288x4096 12.3 us (2.1 TB/s), 5x32000x4096 (f16, groups of 64)
 //   25.5 us (2.7 TB/s, 0.42 of the measured copy rate); without the products the same loads take 4.4, 7.5
-//   and 16 us. Instructions bound it: 300 per pair of units and warp, 130 to 160 of them unpacking,
+//   and 16 us. Instructions bound it: 325 per pair of units and warp in all, 130 to 160 of them unpacking,
 //   loading and multiplying, at 45 % of the issue slots.
 // ------------------------------------------------------------------------------------------
 constexpr int kWarps = 16;

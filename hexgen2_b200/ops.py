@@ -2,7 +2,9 @@
 
 Tensors are passed as raw device pointers plus sizes/strides; every launch goes on torch's
 current CUDA stream. Scratch space (split-K partials, decode split partials) comes from a
-per-device buffer that grows on demand and is reused across calls on the same stream.
+per-device buffer that grows on demand and is reused across calls on the same stream; the
+4-bit operators take a buffer of their own for every call, so that calls on several streams and
+captured graphs never share one.
 """
 from __future__ import annotations
 
